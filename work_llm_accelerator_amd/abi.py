@@ -56,9 +56,27 @@ SIGNATURES: dict[str, list] = {
     + [ctypes.c_float, F32P, c_void_p, c_void_p],
 }
 
+
+
+class Kv8CacheStruct(ctypes.Structure):
+    """qwen_kv8_cache of include/qwen_hip_kv8.h: one layer's codes and scales (device pointers)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("sequences", ctypes.c_int32), ("blocks", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
+class Kv8RowsStruct(ctypes.Structure):
+    """qwen_kv8_rows of include/qwen_hip_kv8.h: rows [sequence][token][head] with strides in elements."""
+
+    _fields_ = [("data", c_void_p), ("seq_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
 # Additive entry points of this build (no counterpart in the reference): the device-resident
 # model API of include/qwen_hip_model.h.  Device pointers are passed as c_void_p.
 P = ctypes.c_void_p
+C8, R8, U64P = ctypes.POINTER(Kv8CacheStruct), ctypes.POINTER(Kv8RowsStruct), ctypes.POINTER(c_u64)
 EXTRA_SIGNATURES: dict[str, tuple[list, object]] = {
     "qwen_hip_last_error": ([], ctypes.c_char_p),
     "qwen_hip_model_create": ([c_int, U8P, F32P, ctypes.POINTER(P)], c_int),
@@ -89,6 +107,14 @@ EXTRA_SIGNATURES: dict[str, tuple[list, object]] = {
     "qwen_hip_fast_project": ([P, P, P, c_int, c_int, P, c_int, c_int, P, P], c_int),
     "qwen_hip_fast_silu_mul_grouped": ([P, P, P, P, P, c_int, P, P, P, P, P], c_int),
     "qwen_hip_fast_project_grouped": ([P, P, c_int, P, P, P, c_int, P, P], c_int),
+    # 8-bit K/V cache (include/qwen_hip_kv8.h)
+    "qwen_hip_kv8_store": ([C8, c_int, R8, R8, c_int, c_int, P, P], c_int),
+    "qwen_hip_kv8_load": ([C8, c_int, R8, R8, c_int, c_int, c_int, P, P], c_int),
+    "qwen_hip_kv8_attention_workspace": ([C8, c_int, c_int, c_int, c_int, c_int, U64P], c_int),
+    "qwen_hip_kv8_attention": ([C8, c_int, R8, R8, c_int, c_int, c_int, P, c_int, ctypes.c_float, P, c_u64, P], c_int),
+    # token sampling (include/qwen_hip_sample.h)
+    "qwen_hip_sample_workspace": ([c_int, c_int, U64P], c_int),
+    "qwen_hip_sample": ([P, c_int, ctypes.c_int64, c_int, c_int, P, P, P, P, P, P, P, c_u64, P], c_int),
     # device-resident descriptor dispatch (include/qwen_hip_dispatch.h): descriptors on the host,
     # DDR images on the device
     "qwen_hip_decode_dispatch_layers": ([c_void_p, c_int, P, P, P, P, P, c_void_p], c_int),

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "qwen_hip_kv8.h"
+
 namespace qwen {
 
 // ---- ORDERED (bit-exact) kernels: kernels_ordered.hip ----
@@ -283,5 +285,38 @@ void run_layer0_reference(const Layer0Weights& W, float eps, bool decode, const 
 size_t head_workspace_bytes(int count, int vocab);
 void launch_head(const float* hidden, int count, const uint16_t* norm_w, const uint16_t* table, int vocab,
                  void* workspace, float* logits, int* ids, hipStream_t st);
+
+// ---- 8-bit K/V cache: kernels_fast_kv8.hip (arguments as in include/qwen_hip_kv8.h, checked by the caller) ----
+constexpr int kKv8Block = QWEN_KV8_BLOCK;
+constexpr int kKv8MaxSplits = 256;
+void launch_kv8_store(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, const qwen_kv8_rows& v, int batch,
+                      int rows, const int* positions, hipStream_t st);
+void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, const qwen_kv8_rows& v, int batch,
+                     int rows, bool zero_outside, const int* positions, hipStream_t st);
+// How an attention call is split: query columns in groups of `tiles` tiles of 16, the keys over nsplit splits of
+// per_split cache blocks, joined by a second launch through `workspace` bytes where nsplit > 1.
+struct Kv8AttnPlan {
+  int tiles, groups, nsplit, per_split;
+  size_t workspace;
+};
+Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys);
+void launch_kv8_attention(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& q, const qwen_kv8_rows& out, int q_heads,
+                          int batch, int rows, const int* positions, int max_keys, float scale, const Kv8AttnPlan& p,
+                          void* workspace, hipStream_t st);
+
+// ---- token sampling: kernels_sample.hip (arguments as in include/qwen_hip_sample.h, checked by the caller) ----
+struct SampleArgs {
+  const void* logits;
+  int type;
+  int64_t row_stride;
+  int rows, vocab;
+  const float *uniforms, *temperature;
+  const int* top_k;
+  const float *top_p, *min_p;
+  int* token_ids;
+};
+constexpr int kSampleMaxVocab = 1 << 24;
+size_t sample_workspace_bytes(int rows, int vocab);
+void launch_sample(const SampleArgs& a, void* workspace, hipStream_t st);
 
 }  // namespace qwen

@@ -1,0 +1,643 @@
+// K/V cache in 8 bits: store, load and the attention over it (code and layout: include/qwen_hip_kv8.h).
+//
+// The codes are exact in fp16, so the matrix cores take them as fp16 operands and the scales, powers of two,
+// are applied to the products: no rounding beside the code's own.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "kernels.hpp"
+#include "qwen_device_math.hpp"
+
+namespace qwen {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+struct Bf16 {  // storage of a bf16 element
+  uint16_t bits;
+};
+
+__device__ __forceinline__ float f32_nan() { return bits_f32(0x7FC00000u); }
+
+// Eight consecutive elements of a 16-byte aligned row.
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const Bf16* p, float (&x)[8]) {
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = bits_f32(w[i] << 16), x[2 * i + 1] = bits_f32(w[i] & 0xFFFF0000u);
+}
+// Round to nearest even; NaN stays a quiet NaN.
+__device__ __forceinline__ uint32_t bf16_of(float x) {
+  const uint32_t b = f32_bits(x);
+  return (b & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(Bf16* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = bf16_of(x[2 * i]) | (bf16_of(x[2 * i + 1]) << 16);
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
+__device__ __forceinline__ void store4(Bf16* p, const f32x4& x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(bf16_of(x[0]) | (bf16_of(x[1]) << 16), bf16_of(x[2]) | (bf16_of(x[3]) << 16));
+}
+
+// 4 x 4 bytes transposed: byte i of o[j] = byte j of w[i].
+__device__ __forceinline__ void transpose4(const uint32_t (&w)[4], uint32_t (&o)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  o[0] = __builtin_amdgcn_perm(c, a, 0x05040100u), o[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  o[2] = __builtin_amdgcn_perm(d, b, 0x05040100u), o[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+__device__ __forceinline__ int code_byte(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+__device__ __forceinline__ uint32_t code_of(float x) { return (uint32_t)(int)rintf(x) & 0xFFu; }
+// The codes of a dword after their block's scale grew by 1 / ratio.
+__device__ __forceinline__ uint32_t regrade(uint32_t w, float ratio) {
+  uint32_t o = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o |= code_of((float)code_byte(w, i) * ratio) << (8 * i);
+  return o;
+}
+
+// ---- store ----------------------------------------------------------------------------------
+// One block of 256 threads per (64-token cache block, head, K or V, sequence): the block's new rows are read once
+// into registers, their largest magnitude gives the scale (a maximum of bit patterns: non-finite values come
+// out on top), and the codes are written once; V goes through LDS to turn 4 x 4 bytes.  The earlier rows of a
+// part-filled block are read only where the scale grows.  Bound by the stream of new rows.
+// grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
+template <class T, int D>
+__global__ void __launch_bounds__(256) kv8_store_kernel(qwen_kv8_cache c, qwen_kv8_rows kin, qwen_kv8_rows vin, int rows,
+                                                        const int* __restrict__ positions) {
+  constexpr int kPer = D / 8;               // threads of a row
+  constexpr int kStep = 256 / kPer;         // rows of a pass
+  constexpr int kPasses = kKv8Block / kStep;
+  __shared__ uint32_t red[4];
+  __shared__ uint32_t tile[kKv8Block][D / 4 + 2];
+  const int b = blockIdx.z, h = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  const int pos = positions[b];
+  if (pos < 0) return;
+  const int blk = pos / kKv8Block + (int)blockIdx.x;
+  if (blk >= c.blocks) return;
+  const long long end = (long long)pos + rows - (long long)blk * kKv8Block;
+  if (end <= 0) return;
+  const int t0 = blockIdx.x == 0 ? pos % kKv8Block : 0, t1 = end < kKv8Block ? (int)end : kKv8Block;
+  const long long first = (long long)blk * kKv8Block - pos;  // row of the block's token 0
+  const qwen_kv8_rows in = is_v ? vin : kin;
+  const T* src = static_cast<const T*>(in.data) + b * in.seq_stride + h * in.head_stride;
+  const int tid = threadIdx.x, d8 = (tid % kPer) * 8;
+  float x[kPasses][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = p * kStep + tid / kPer;
+    if (t >= t0 && t < t1) {
+      load8(src + (first + t) * in.token_stride + d8, x[p]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, f32_bits(x[p][e]) & 0x7FFFFFFFu);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[p][e] = 0.0f;
+    }
+  }
+  const size_t place = ((size_t)b * c.blocks + blk) * c.kv_heads + h;
+  float* scale_at = (is_v ? c.v_scale : c.k_scale) + place;
+  const float old = t0 > 0 ? *scale_at : 0.0f;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  // 127 = 1.7E0000 (hex mantissa) * 2^6: the exponent of the least power of two, biased by 127
+  const int e = max(1, (int)(top >> 23) - ((top & 0x7FFFFFu) > 0x7E0000u ? 5 : 6));
+  float s = bits_f32((uint32_t)e << 23);
+  if (t0 > 0) s = old > s || old != old ? old : s;
+  if (top >= 0x7F800000u) s = f32_nan();
+  const bool finite = s == s;
+  const float inv = finite ? 1.0f / s : 0.0f;
+  const bool grown = t0 > 0 && finite && s != old;
+  const float ratio = grown ? old * inv : 1.0f;
+  if (tid == 0) *scale_at = s;
+  uint2 code[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    uint32_t w[2] = {0u, 0u};
+    if (finite) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i >> 2] |= code_of(x[p][i] * inv) << (8 * (i & 3));
+    }
+    code[p] = make_uint2(w[0], w[1]);
+  }
+  int8_t* dst = (is_v ? c.v : c.k) + place * (size_t)(kKv8Block * D);
+  if (!is_v) {
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int t = p * kStep + tid / kPer;
+      uint2* at = reinterpret_cast<uint2*>(dst + ((d8 >> 6) * kKv8Block + t) * 64 + (d8 & 63));
+      if (t >= t0 && t < t1) {
+        *at = code[p];
+      } else if (t < t0 && grown) {
+        const uint2 w = *at;
+        *at = make_uint2(regrade(w.x, ratio), regrade(w.y, ratio));
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = p * kStep + tid / kPer;
+    tile[t][d8 / 4] = code[p].x;
+    tile[t][d8 / 4 + 1] = code[p].y;
+  }
+  __syncthreads();
+  // thread: dimensions 4 d4 .. + 3, tokens 16 (2 half + u) + 4 g .. + 3 for u = 0, 1 (eight adjacent bytes)
+  const int half = tid & 1, g = (tid >> 1) & 3, d4 = tid >> 3;
+  if (d4 >= D / 4) return;
+  uint32_t o[2][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = 16 * (2 * half + u) + 4 * g;
+    const uint32_t w[4] = {tile[t][d4], tile[t + 1][d4], tile[t + 2][d4], tile[t + 3][d4]};
+    transpose4(w, o[u]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t* at = reinterpret_cast<uint32_t*>(dst + (4 * d4 + j) * kKv8Block + 16 * g + 8 * half);
+    if (t0 == 0 && t1 == kKv8Block) {
+      *reinterpret_cast<uint2*>(at) = make_uint2(o[0][j], o[1][j]);
+      continue;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = 16 * (2 * half + u) + 4 * g;
+      const bool any_new = t < t1 && t + 4 > t0, any_old = t < t0;
+      if (!any_new && !(any_old && grown)) continue;
+      const uint32_t was = at[u], re = grown ? regrade(was, ratio) : was;
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w |= (t + i < t0 ? re : t + i < t1 ? o[u][j] : was) & (0xFFu << (8 * i));
+      at[u] = w;
+    }
+  }
+}
+
+// ---- load -----------------------------------------------------------------------------------
+// The inverse, one block of 256 threads per (cache block, head, K or V, sequence); bound by the rows written.
+// grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
+template <class T, int D>
+__global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv8_rows kout, qwen_kv8_rows vout, int rows,
+                                                       int zero_outside, const int* __restrict__ positions) {
+  constexpr int kPer = D / 8, kStep = 256 / kPer, kPasses = kKv8Block / kStep;
+  __shared__ uint32_t tile[kKv8Block][D / 4 + 2];
+  const int b = blockIdx.z, h = blockIdx.y >> 1;
+  const bool is_v = blockIdx.y & 1;
+  const int pos = positions[b];
+  const long long blk = (long long)(pos >> 6) + blockIdx.x;  // rounds down for negative positions too
+  const bool inside = blk >= 0 && blk < c.blocks;
+  if (!inside && !zero_outside) return;
+  const long long first = blk * kKv8Block - pos, last = first + kKv8Block;  // rows of the block's tokens
+  if (first >= rows) return;
+  const int t0 = first < 0 ? (int)-first : 0, t1 = last > rows ? (int)(rows - first) : kKv8Block;
+  const qwen_kv8_rows out = is_v ? vout : kout;
+  T* dst = static_cast<T*>(out.data) + b * out.seq_stride + h * out.head_stride;
+  const int tid = threadIdx.x, d8 = (tid % kPer) * 8;
+  const size_t place = inside ? ((size_t)b * c.blocks + (size_t)blk) * c.kv_heads + h : 0;
+  const int8_t* src = (is_v ? c.v : c.k) + place * (size_t)(kKv8Block * D);
+  const float s = inside ? (is_v ? c.v_scale : c.k_scale)[place] : 0.0f;
+  if (is_v && inside) {
+    const int half = tid & 1, g = (tid >> 1) & 3, d4 = tid >> 3;
+    if (d4 < D / 4) {
+      uint2 in[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        in[j] = *reinterpret_cast<const uint2*>(src + (4 * d4 + j) * kKv8Block + 16 * g + 8 * half);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = 16 * (2 * half + u) + 4 * g;
+        const uint32_t w[4] = {u ? in[0].y : in[0].x, u ? in[1].y : in[1].x, u ? in[2].y : in[2].x, u ? in[3].y : in[3].x};
+        uint32_t o[4];
+        transpose4(w, o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tile[t + i][d4] = o[i];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int t = p * kStep + tid / kPer;
+    if (t < t0 || t >= t1) continue;
+    uint2 w = make_uint2(0u, 0u);
+    if (inside) {
+      if (is_v)
+        w = make_uint2(tile[t][d8 / 4], tile[t][d8 / 4 + 1]);
+      else
+        w = *reinterpret_cast<const uint2*>(src + ((d8 >> 6) * kKv8Block + t) * 64 + (d8 & 63));
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)code_byte(i < 4 ? w.x : w.y, i & 3) * s;
+    store8(dst + (first + t) * out.token_stride + d8, x);
+  }
+}
+
+// ---- attention ------------------------------------------------------------------------------
+struct Kv8AttnArgs {
+  qwen_kv8_cache c;
+  qwen_kv8_rows q, out;
+  const int* positions;
+  int group, rows, max_keys;
+  float scale_log2e;
+  int nsplit, per_split;  // key splits of `per_split` blocks
+  float* part;            // [batch][kv_heads][rows * group][nsplit][D], nsplit > 1
+  float2* pml;            // [batch][kv_heads][rows * group][nsplit]
+};
+
+// Eight codes as fp16: 0x64uu is 1024 + uu, uu = code + 128.
+__device__ __forceinline__ half8 codes_to_half(uint32_t lo, uint32_t hi) {
+  const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
+  const uint32_t w[4] = {
+      __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u),
+      __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
+  half8 r;
+  __builtin_memcpy(&r, w, 16);
+  return r - (_Float16)1152.0f;
+}
+
+// The value of the lane whose column differs by 8 (row_ror:8).
+__device__ __forceinline__ float other_half(float x) {
+  return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), 0x128, 0xF, 0xF, false));
+}
+
+constexpr float kProbBits = 15.0f;  // probabilities times 2^15: fp16 holds them normal down to 2^-29 of the largest
+
+// Attention of CT tiles of 16 query columns over one split of the keys.  Per wave and 64-token block:
+//   S^T = K Q^T (16x16x32 fp16, A = the codes of 16 tokens as they lie in the cache, B = query columns), so a lane
+//   holds the scores of one column for tokens 16t + 4g + i: exactly the k slots of the B operand of
+//   O^T += V P^T, whose A operand is again 16 contiguous cache bytes a lane.  Scores and probabilities never leave
+//   their lane; K and V go from HBM to the matrix cores through registers alone, with the next block's loads in
+//   flight.  Running maximum and sum per column; the waves of a block take its cache blocks in turn and are
+//   joined in LDS.
+// fp32 queries take two columns each (hi and lo fp16 terms, 8 apart), whose scores are added across lanes; the
+// columns then carry the hi and lo terms of the probabilities.
+// grid = (nsplit * tile groups, kv_heads, batch), block = 256.
+template <class T, int D, int CT>
+__global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
+  constexpr bool kTwo = std::is_same<T, float>::value;
+  constexpr int kRowsPerTile = kTwo ? 8 : 16, kHalves = D / 64, kDimTiles = D / 16;
+  __shared__ float2 ml[4][CT * 16];
+  __shared__ f32x4 join[2][CT][kDimTiles][64];
+  const int split = blockIdx.x % a.nsplit, groups = gridDim.x / a.nsplit;
+  const int tg = groups - 1 - (int)(blockIdx.x / a.nsplit);  // the longest rows first
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int R = a.rows * a.group, row0 = tg * CT * kRowsPerTile;
+  const int pos = a.positions[b];
+  // keys that the first and the last row of the tile group attend
+  const int i_last = min(R - 1, row0 + CT * kRowsPerTile - 1) / a.group;
+  auto visible = [&](int i) { return pos < 0 ? 0 : (int)min((long long)pos + i + 1, (long long)a.max_keys); };
+  const int kmin = visible(row0 / a.group), kmax = visible(i_last);
+  const int nblk = (kmax + kKv8Block - 1) / kKv8Block;
+  const int blk0 = split * a.per_split, blk1 = min(nblk, blk0 + a.per_split);
+  if (blk0 >= blk1 && a.nsplit > 1) return;  // the merge knows the live splits
+
+  // Query columns
+  half8 q[CT][2 * kHalves];
+  float factor[CT], m[CT], l[CT];
+  int keys[CT];
+  f32x4 o[CT][kDimTiles];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int row = row0 + ct * kRowsPerTile + (kTwo ? col & 7 : col);
+    const bool live = row < R;
+    const int i = live ? row / a.group : 0, h = kvh * a.group + (live ? row % a.group : 0);
+    const T* src = static_cast<const T*>(a.q.data) + b * a.q.seq_stride + (long long)i * a.q.token_stride +
+                   (long long)h * a.q.head_stride;
+    keys[ct] = live ? visible(i) : 0;
+    float x[2 * kHalves][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < 2 * kHalves; ++s) {
+      load8(src + 64 * (s >> 1) + 16 * g + 8 * (s & 1), x[s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, f32_bits(x[s][e]) & 0x7FFFFFFFu);
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    // times a power of two that brings the row's largest magnitude to [2^13, 2^14)
+    const int ex = min(253, max(13, 267 - (int)(top >> 23)));
+    const float up = bits_f32((uint32_t)ex << 23);
+    factor[ct] = top >= 0x7F800000u ? f32_nan() : a.scale_log2e * bits_f32((uint32_t)(254 - ex) << 23);
+#pragma unroll
+    for (int s = 0; s < 2 * kHalves; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = x[s][e] * up;
+        const _Float16 hi = (_Float16)y;
+        q[ct][s][e] = kTwo && col >= 8 ? (_Float16)(y - (float)hi) : hi;
+      }
+    m[ct] = -__builtin_inff();
+    l[ct] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const size_t block_bytes = (size_t)kKv8Block * D, head0 = (size_t)b * a.c.blocks * a.c.kv_heads + kvh;
+  uint4 kr[4][kHalves], vr[kDimTiles];
+  auto load_k = [&](int blk) {
+    const int8_t* p = a.c.k + (head0 + (size_t)blk * a.c.kv_heads) * block_bytes + col * 64 + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int s = 0; s < kHalves; ++s) kr[t][s] = *reinterpret_cast<const uint4*>(p + (s * kKv8Block + 16 * t) * 64);
+  };
+  auto load_v = [&](int blk) {
+    const int8_t* p = a.c.v + (head0 + (size_t)blk * a.c.kv_heads) * block_bytes + col * 64 + 16 * g;
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(p + dt * 16 * kKv8Block);
+  };
+  int blk = blk0 + wave;
+  float sk = 0.0f, sv = 0.0f;
+  if (blk < blk1) {
+    load_k(blk);
+    load_v(blk);
+    sk = a.c.k_scale[head0 + (size_t)blk * a.c.kv_heads];
+    sv = a.c.v_scale[head0 + (size_t)blk * a.c.kv_heads];
+  }
+  for (; blk < blk1; blk += 4) {
+    const int next = min(blk + 4, blk1 - 1);  // past the end: a block of the split again (not used)
+    f32x4 s[CT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < kHalves; ++u) {
+        const half8 k0 = codes_to_half(kr[t][u].x, kr[t][u].y), k1 = codes_to_half(kr[t][u].z, kr[t][u].w);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[ct][2 * u], s[ct][t], 0, 0, 0);
+          s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[ct][2 * u + 1], s[ct][t], 0, 0, 0);
+        }
+      }
+    }
+    load_k(next);
+    const float sk_next = a.c.k_scale[head0 + (size_t)next * a.c.kv_heads];
+    const bool edge = (blk + 1) * kKv8Block > kmin;
+    half8 p[CT][2];
+    float sv_col[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float f = factor[ct] * sk;
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s[ct][t][i];
+          if constexpr (kTwo) x += other_half(x);
+          x *= f;
+          if (edge && blk * kKv8Block + 16 * t + 4 * g + i >= keys[ct]) x = -__builtin_inff();
+          s[ct][t][i] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      // a column that attends none of the block's tokens takes nothing from it, whatever its scale holds
+      sv_col[ct] = top == -__builtin_inff() ? 0.0f : sv;
+      const float mn = fmaxf(m[ct], top);
+      if (__any(mn > m[ct])) {
+        const float alpha = mn > m[ct] ? exp2f(m[ct] - mn) : 1.0f;
+        l[ct] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] *= alpha;
+        m[ct] = mn;
+      }
+      const float base = m[ct] == -__builtin_inff() ? 0.0f : m[ct] - kProbBits;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = __builtin_amdgcn_exp2f(s[ct][t][i] - base);
+          l[ct] += x;
+          const _Float16 hi = (_Float16)x;
+          p[ct][t >> 1][4 * (t & 1) + i] = kTwo && col >= 8 ? (_Float16)(x - (float)hi) : hi;
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt) {
+      const half8 v0 = codes_to_half(vr[dt].x, vr[dt].y), v1 = codes_to_half(vr[dt].z, vr[dt].w);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[ct][0], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[ct][1], d, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[ct][dt][i] = fmaf(d[i], sv_col[ct], o[ct][dt][i]);
+      }
+    }
+    load_v(next);
+    sv = a.c.v_scale[head0 + (size_t)next * a.c.kv_heads];
+    sk = sk_next;
+  }
+
+  // Join the waves: common maximum, then two halves in LDS
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16, 64);
+    l[ct] += __shfl_xor(l[ct], 32, 64);
+    if (g == 0) ml[wave][ct * 16 + col] = make_float2(m[ct], l[ct]);
+  }
+  __syncthreads();
+  float total[CT], most[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float mm = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w][ct * 16 + col].x);
+    total[ct] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 v = ml[w][ct * 16 + col];
+      // (a wave without keys: maximum -inf and sum 0; a sum of NaN stays one)
+      total[ct] += v.x == -__builtin_inff() ? v.y : v.y * exp2f(v.x - mm);
+    }
+    const float f = m[ct] == -__builtin_inff() ? 1.0f : exp2f(m[ct] - mm);
+#pragma unroll
+    for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] *= f;
+    most[ct] = mm;
+  }
+#pragma unroll
+  for (int step = 2; step > 0; step >>= 1) {
+    if (wave >= step && wave < 2 * step)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int dt = 0; dt < kDimTiles; ++dt) join[wave - step][ct][dt][lane] = o[ct][dt];
+    __syncthreads();
+    if (wave < step)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] += join[wave][ct][dt][lane];
+    __syncthreads();
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int row = row0 + ct * kRowsPerTile + (kTwo ? col & 7 : col);
+    if constexpr (kTwo)
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[ct][dt][i] += other_half(o[ct][dt][i]);
+    if (row >= R || (kTwo && col >= 8)) continue;
+    if (a.nsplit > 1) {
+      const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit + split;
+      if (g == 0) a.pml[at] = make_float2(most[ct], total[ct]);
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt) store4(a.part + at * D + 16 * dt + 4 * g, o[ct][dt]);
+    } else {
+      const float inv = total[ct] == 0.0f ? 0.0f : 1.0f / total[ct];
+      T* dst = static_cast<T*>(a.out.data) + b * a.out.seq_stride + (long long)(row / a.group) * a.out.token_stride +
+               (long long)(kvh * a.group + row % a.group) * a.out.head_stride;
+#pragma unroll
+      for (int dt = 0; dt < kDimTiles; ++dt) store4(dst + 16 * dt + 4 * g, o[ct][dt] * inv);
+    }
+  }
+}
+
+// Joins the key splits of one query row: grid = (rows * group, kv_heads, batch), block = D.
+template <class T, int D, int RT>
+__global__ void __launch_bounds__(D) kv8_merge_kernel(Kv8AttnArgs a) {
+  const int row = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, R = a.rows * a.group;
+  const int pos = a.positions[b];
+  // live splits: those of the row's tile group (RT rows), as kv8_attn_kernel counts them
+  const int i_last = min(R - 1, row / RT * RT + RT - 1) / a.group;
+  const int kmax = pos < 0 ? 0 : (int)min((long long)pos + i_last + 1, (long long)a.max_keys);
+  const int live = ((kmax + kKv8Block - 1) / kKv8Block + a.per_split - 1) / a.per_split;
+  const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit;
+  float mm = -__builtin_inff();
+  for (int s = 0; s < live; ++s) mm = fmaxf(mm, a.pml[at + s].x);
+  float sum = 0.0f, o = 0.0f;
+  for (int s = 0; s < live; ++s) {
+    const float2 v = a.pml[at + s];
+    const float f = v.x == -__builtin_inff() ? 1.0f : exp2f(v.x - mm);
+    sum += v.y * f;
+    o = fmaf(a.part[(at + s) * D + threadIdx.x], f, o);
+  }
+  const float y = sum == 0.0f ? 0.0f : o * (1.0f / sum);
+  T* dst = static_cast<T*>(a.out.data) + b * a.out.seq_stride + (long long)(row / a.group) * a.out.token_stride +
+           (long long)(kvh * a.group + row % a.group) * a.out.head_stride + threadIdx.x;
+  if constexpr (std::is_same<T, float>::value)
+    *dst = y;
+  else
+    dst->bits = (uint16_t)bf16_of(y);
+}
+
+template <class T, int D, int CT>
+void run_attn(const Kv8AttnArgs& a, int batch, int groups, hipStream_t st) {
+  constexpr int kRows = CT * (std::is_same<T, float>::value ? 8 : 16);
+  hipLaunchKernelGGL((kv8_attn_kernel<T, D, CT>), dim3(a.nsplit * groups, a.c.kv_heads, batch), dim3(256), 0, st, a);
+  if (a.nsplit > 1)
+    hipLaunchKernelGGL((kv8_merge_kernel<T, D, kRows>), dim3(a.rows * a.group, a.c.kv_heads, batch), dim3(D), 0, st, a);
+}
+template <class T, int D>
+void run_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int batch, hipStream_t st) {
+  if (p.tiles == 1)
+    run_attn<T, D, 1>(a, batch, p.groups, st);
+  else if (p.tiles == 2)
+    run_attn<T, D, 2>(a, batch, p.groups, st);
+  else
+    run_attn<T, D, 4>(a, batch, p.groups, st);
+}
+
+template <class F>
+void by_type(int type, int head_dim, F&& f) {
+  if (type == QWEN_TYPE_F32) {
+    if (head_dim == 64)
+      f(float{}, std::integral_constant<int, 64>{});
+    else
+      f(float{}, std::integral_constant<int, 128>{});
+  } else {
+    if (head_dim == 64)
+      f(Bf16{}, std::integral_constant<int, 64>{});
+    else
+      f(Bf16{}, std::integral_constant<int, 128>{});
+  }
+}
+
+}  // namespace
+
+void launch_kv8_store(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, const qwen_kv8_rows& v, int batch,
+                      int rows, const int* positions, hipStream_t st) {
+  const int touched = (rows + kKv8Block - 2) / kKv8Block + 1;
+  by_type(type, c.head_dim, [&](auto t, auto d) {
+    hipLaunchKernelGGL((kv8_store_kernel<decltype(t), decltype(d)::value>), dim3(touched, 2 * c.kv_heads, batch),
+                       dim3(256), 0, st, c, k, v, rows, positions);
+  });
+}
+
+void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, const qwen_kv8_rows& v, int batch,
+                     int rows, bool zero_outside, const int* positions, hipStream_t st) {
+  const int touched = (rows + kKv8Block - 2) / kKv8Block + 1;
+  by_type(type, c.head_dim, [&](auto t, auto d) {
+    hipLaunchKernelGGL((kv8_load_kernel<decltype(t), decltype(d)::value>), dim3(touched, 2 * c.kv_heads, batch),
+                       dim3(256), 0, st, c, k, v, rows, (int)zero_outside, positions);
+  });
+}
+
+Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys) {
+  const int group = q_heads / c.kv_heads, per_tile = type == QWEN_TYPE_F32 ? 8 : 16;
+  const long long tiles = ((long long)rows * group + per_tile - 1) / per_tile;
+  Kv8AttnPlan p{};
+  p.tiles = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+  p.groups = (int)((tiles + p.tiles - 1) / p.tiles);
+  const long long blocks = (max_keys + kKv8Block - 1) / kKv8Block;
+  const long long others = (long long)p.groups * c.kv_heads * batch;
+  long long per = (blocks * others + 511) / 512;
+  if (per < 4) per = 4;
+  const long long least = (blocks + kKv8MaxSplits - 1) / kKv8MaxSplits;
+  if (per < least) per = least;
+  per = (per + 3) / 4 * 4;
+  p.per_split = (int)per;
+  p.nsplit = (int)((blocks + per - 1) / per);
+  if (p.nsplit > 1)
+    p.workspace = (size_t)batch * q_heads * rows * p.nsplit * (size_t)(c.head_dim + 2) * sizeof(float);
+  return p;
+}
+
+void launch_kv8_attention(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& q, const qwen_kv8_rows& out, int q_heads,
+                          int batch, int rows, const int* positions, int max_keys, float scale, const Kv8AttnPlan& p,
+                          void* workspace, hipStream_t st) {
+  Kv8AttnArgs a{};
+  a.c = c;
+  a.q = q;
+  a.out = out;
+  a.positions = positions;
+  a.group = q_heads / c.kv_heads;
+  a.rows = rows;
+  a.max_keys = max_keys;
+  a.scale_log2e = scale * 1.44269504088896340736f;
+  a.nsplit = p.nsplit;
+  a.per_split = p.per_split;
+  a.part = static_cast<float*>(workspace);
+  a.pml = reinterpret_cast<float2*>(a.part + (size_t)batch * q_heads * rows * p.nsplit * c.head_dim);
+  by_type(type, c.head_dim, [&](auto t, auto d) { run_attn<decltype(t), decltype(d)::value>(a, p, batch, st); });
+}
+
+}  // namespace qwen

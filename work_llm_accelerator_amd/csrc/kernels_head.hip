@@ -34,14 +34,6 @@ __device__ __forceinline__ float to_bf16(float x) {
 }
 __device__ __forceinline__ uint16_t f32_to_bf16_bits(float x) { return (uint16_t)(f32_bits(to_bf16(x)) >> 16); }
 
-// Total order of floats for the argmax key: larger value -> larger key, -0 == +0, NaN above all.
-__device__ __forceinline__ uint32_t order_key(float f) {
-  uint32_t b = f32_bits(f);
-  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
-  if (b == 0x80000000u) b = 0u;
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
 // One block per row (rows_padded, a multiple of 16); rows >= count are written as zeros so the
 // lm_head can stage whole 16-row tiles.  block = 256 (6 values per thread).
 __global__ void __launch_bounds__(256) head_norm_kernel(const float* __restrict__ x, int count,

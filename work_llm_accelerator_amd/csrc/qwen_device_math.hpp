@@ -134,6 +134,14 @@ QWEN_HD float silu_prefill(float v) { return v / (1.0f + approx_exp(-v)); }     
 QWEN_HD int nibble_lo(uint32_t b) { return (int)((b & 0xFu) ^ 8u) - 8; }
 QWEN_HD int nibble_hi(uint32_t b) { return (int)(((b >> 4) & 0xFu) ^ 8u) - 8; }
 
+// Total order of floats for the argmax key: larger value -> larger key, -0 == +0, NaN above all.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  uint32_t b = f32_bits(f);
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
+  if (b == 0x80000000u) b = 0u;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
 // bf16 rounding of the driver (verification/reference_wrapper_backend.py:40-46), uint32 wrap-around.
 QWEN_HD float round_bf16(float x) {
   uint32_t b = f32_bits(x);
