@@ -16,8 +16,8 @@
  *   5. of those, the ones with w_i >= min(q, 1) (all, when q <= 0 or NaN).
  *   6. The token is the lowest index i at which the sum of the kept weights up to and including i exceeds u
  *      times their total (u clamped to [0, 1], NaN as 0; the last kept token where none does).
- * exp is taken in 64 bits and each weight rounded to a multiple of 2^-(62 - ceil(log2 vocab)) (2^-44 for 151936
- * tokens), so all sums are exact integers: the result does not depend on the order in which they are formed.
+ * exp is taken in 64 bits and each weight rounded to a multiple of 2^-min(50, 62 - ceil(log2 vocab)) (2^-44 for
+ * 151936 tokens), so all sums are exact integers: the result does not depend on the order in which they are formed.
  *
  * All data pointers are DEVICE pointers; work is queued on `stream` (a hipStream_t of the current device, 0 for
  * the null stream), nothing is allocated or synchronized, and the call can be captured into a graph.  Calls
@@ -36,7 +36,7 @@ extern "C" {
 /* Bytes of workspace that qwen_hip_sample needs. */
 int qwen_hip_sample_workspace(int rows, int vocab, uint64_t* bytes);
 
-/* logits: `rows` rows of `vocab` (1 .. 2^24) values of `type` (QWEN_TYPE_F32 or QWEN_TYPE_BF16 of
+/* logits: `rows` (1 .. 65535) rows of `vocab` (1 .. 2^24) values of `type` (QWEN_TYPE_F32 or QWEN_TYPE_BF16 of
  * qwen_hip_kv8.h), row r at r * row_stride elements.  uniforms [rows] fp32; temperature, top_p, min_p [rows]
  * fp32 and top_k [rows] int32, each may be null (1, off, off, off).  token_ids [rows] int32.  workspace
  * 16-byte aligned, contents need not be kept. */

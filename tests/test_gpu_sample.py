@@ -26,7 +26,7 @@ def drawn(x, u, t=1.0, k=0, p=1.0, q=0.0) -> int:
     top = x.max()
     if not t > 0 or not np.isfinite(top):
         return int(np.argmax(x))
-    unit = 2.0 ** (62 - max(0, math.ceil(math.log2(len(x)))))
+    unit = 2.0 ** min(50, 62 - math.ceil(math.log2(len(x))))
     w = np.exp((x - top) / np.float64(t))
     n = [int(v) for v in np.rint(w * unit)]
     order = np.lexsort((np.arange(len(x)), -x))
@@ -198,3 +198,26 @@ def test_graph_replays(torch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(ids, sample_logits(x, u, top_p=p, top_k=k))
+
+
+def test_cuts_in_crowded_steps(torch):
+    """Rows whose cut falls among thousands of logits that are equal or nearly so, rows of a few distinct values far
+    apart, masks of -inf and of the lowest value, and a long flat tail without weight."""
+    rng = np.random.default_rng(8)
+    rows, vocab = 10, 20000
+    x = np.zeros((rows, vocab), np.float32)
+    x[0] = rng.standard_normal(vocab) * 1e-6
+    x[0, 7] = 20.0
+    x[1, ::3] = -30.0
+    x[2] = np.where(rng.random(vocab) < 0.7, -np.inf, rng.standard_normal(vocab))
+    x[3] = np.where(rng.random(vocab) < 0.7, np.finfo(np.float32).min, rng.standard_normal(vocab))
+    x[4] = np.floor(rng.random(vocab) * 4) * 1e4
+    x[5] = rng.standard_normal(vocab) - 60.0
+    x[5, 3] = 0.0
+    x[6] = 1e-40 * rng.integers(0, 9, vocab)
+    x[7] = np.nextafter(np.float32(1), np.float32(2)) * (rng.random(vocab) < 0.5)
+    x[8] = 3e38 * (2 * rng.random(vocab) - 1)
+    x[9] = rng.standard_normal(vocab) * 3
+    for k, p in ((0, 0.5), (15000, 1.0), (15000, 0.3), (9000, 0.999), (1, 0.5), (5000, 0.9999)):
+        for t in (1.0, 0.05, 30.0):
+            check(torch, x, rng.random(rows), temperature=[t] * rows, top_k=[k] * rows, top_p=[p] * rows)

@@ -87,7 +87,7 @@ def sample(lib, logits=PTR, kind=0, stride=100, n=2, vocab=100, u=PTR, ids=PTR, 
 
 
 @pytest.mark.parametrize("bad", [dict(logits=None), dict(u=None), dict(ids=None), dict(kind=2), dict(n=0), dict(n=-1),
-                                 dict(n=(1 << 20) + 1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(stride=-1),
+                                 dict(n=65536), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(stride=-1),
                                  dict(stride=1 << 41), dict(logits=PTR + 2), dict(kind=1, logits=PTR + 1)])
 def test_sample_refuses(lib, bad):
     assert sample(lib, **bad) == 1

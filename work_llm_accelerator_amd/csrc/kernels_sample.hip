@@ -1,9 +1,13 @@
 // Token sampling (semantics: include/qwen_hip_sample.h).
 //
 // Nothing is sorted.  Tokens are ranked by a 32-bit key of their logit (order_key: larger value, larger key) with
-// ties by index, so a kept set is {key > T} and the first n of {key == T}: top-k and top-p each find their (T, n)
-// by three radix steps (11, 11 and 10 bits) over histograms of counts or weights, min-p is a test per token.
-// Weights are 64-bit integers (fixed point), so histogram sums are exact whatever the order of their atomics.
+// ties by index, so a kept set is {key > T} and the first n of {key == T}; min-p is a test per token.  Weights are
+// 64-bit integers (fixed point), so sums are exact whatever the order of their atomics.
+//
+// Six launches, each over all rows: the row's maximum and minimum; a histogram (counts and weights) over 2048 equal
+// steps of the logit below the maximum; a list of the tokens of the steps in which top-k and top-p cut; the exact
+// (T, n) from that list; the kept weight of each segment of the row; the draw.  Rows are split over many blocks
+// except in the two launches that end in one number (the cut and the draw).
 #include <hip/hip_runtime.h>
 
 #include "kernels.hpp"
@@ -15,7 +19,12 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kBuckets = 2048;
-constexpr int kSegments = 1024;  // most index ranges of a row in the draw
+constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row)
+constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kThreads * 512 tokens)
+constexpr int kMaxChunks = 256;
+constexpr uint32_t kUnlisted = 0xFFFFFFFFu;
+constexpr int kChunkThreads = 256;
+constexpr int kHistThreads = 512;
 
 __device__ __forceinline__ float logit_at(const float* p, int i) { return p[i]; }
 __device__ __forceinline__ float logit_at(const uint16_t* p, int i) { return bits_f32((uint32_t)p[i] << 16); }
@@ -30,7 +39,8 @@ struct Cut {       // a kept set: key > key, and the first `ties` tokens with ke
   uint32_t ties;
 };
 
-// Sum over the block's 1024 threads and the sums of the threads before (exclusive).
+// Sum over the block's threads (N) and the sum of the threads before (exclusive).
+template <int N>
 __device__ u64 block_scan(u64 x, u64* red, u64& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   u64 inc = x;
@@ -44,7 +54,8 @@ __device__ u64 block_scan(u64 x, u64* red, u64& total) {
   __syncthreads();
   u64 before = 0;
   total = 0;
-  for (int w = 0; w < kThreads / 64; ++w) {
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) {
     const u64 v = red[w];
     before += w < wave ? v : 0ull;
     total += v;
@@ -52,220 +63,672 @@ __device__ u64 block_scan(u64 x, u64* red, u64& total) {
   return before + inc - x;
 }
 
-// One block per row.
-template <class T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(SampleArgs a, double unit) {
-  __shared__ u64 hist[kBuckets];
-  __shared__ uint32_t count[kBuckets];
-  __shared__ u64 red[kThreads / 64];
-  __shared__ u64 pick_above;
-  __shared__ uint32_t pick_bucket, pick_count_above;
-  const int row = blockIdx.x, tid = threadIdx.x, vocab = a.vocab;
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+// One row's workspace.
+struct RowSpace {
+  u64 weights[kBuckets];      // histogram
+  uint32_t counts[kBuckets];
+  u64 best[kMaxChunks];       // (key << 32 | ~index) of each chunk's maximum
+  float low[kMaxChunks];      // least finite logit
+  uint32_t list[kList];       // keys of the tokens of the steps with a cut
+  uint32_t listed;
+  int k_step, p_low, p_high;  // the steps in the list (Needed)
+  u64 k_before;
+  Cut cut;
+};
 
-  // maximum and its first index
-  u64 best = 0;
-  for (int i = tid; i < vocab; i += kThreads) {
-    const u64 k = ((u64)order_key(logit_at(x, i)) << 32) | (u64)(~(uint32_t)i);
-    best = k > best ? k : best;
+struct Sampler {
+  SampleArgs a;
+  int unit_bits;  // the weight of the largest logit is 2^unit_bits
+  float spread;   // logits further than spread * temperature below the maximum have weight 0
+  int chunks, per_chunk;            // blocks that share a row: maxima,
+  int hist_chunks, hist_per_chunk;  // histogram and list
+  int segments, blocks_per_segment;  // of kSegment tokens
+  RowSpace* space;
+  u64* seg_weight;     // [rows][segments]
+  uint32_t* seg_ties;  // [rows][segments]
+};
+
+// 2^(t + bits) for t <= 0, 0 where t is below -110: Taylor's series over half a binade each way, degree 12 (its remainder
+// is below 2^-52 of the value), the exponent set by integer addition.  (About a third of the operations of the
+// library's exp, a division and a conversion to 64-bit integers, which were most of the histogram's time.)
+__device__ __forceinline__ double exp2_falling(double t, int bits) {
+  constexpr double kLn2 = 0.693147180559945309417232121458, kMagic = 6755399441055744.0;  // 1.5 * 2^52
+  constexpr double c2 = kLn2 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5, c6 = c5 * kLn2 / 6,
+                   c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10, c11 = c10 * kLn2 / 11,
+                   c12 = c11 * kLn2 / 12;
+  const bool tiny = !(t >= -110.0);  // (NaN too: -inf logits at an infinite temperature)
+  t = tiny ? -110.0 : t;
+  const double m = t + kMagic, f = t - (m - kMagic);  // the low word of m is rint(t)
+  double p = fma(c12, f, c11);
+  p = fma(p, f, c10);
+  p = fma(p, f, c9);
+  p = fma(p, f, c8);
+  p = fma(p, f, c7);
+  p = fma(p, f, c6);
+  p = fma(p, f, c5);
+  p = fma(p, f, c4);
+  p = fma(p, f, c3);
+  p = fma(p, f, c2);
+  p = fma(p, f, kLn2);
+  p = fma(p, f, 1.0);
+  const int k = (int)(uint32_t)__double_as_longlong(m) + bits;
+  return tiny ? 0.0 : __hiloint2double(__double2hiint(p) + (k << 20), __double2loint(p));
+}
+// rint(x) for 0 <= x < 2^51.
+__device__ __forceinline__ u64 rint_u64(double x) {
+  constexpr double kMagic = 4503599627370496.0;  // 2^52
+  return (u64)__double_as_longlong(x + kMagic) & 0xFFFFFFFFFFFFFull;
+}
+
+// What every launch after the first derives from the chunks' maxima.
+struct Row {
+  uint32_t top_key;
+  int top_index;
+  float top, temperature;
+  float steps;  // histogram steps per unit of the logit
+  double dtop, per_unit;  // per_unit: log2(e) / temperature
+  int unit_bits;
+  bool greedy;
+
+  // Whole blocks of at least 256 threads (a multiple of 64); red: one u64 and one float per wave.
+  __device__ Row(const Sampler& s, int row, u64* red, float* redf) {
+    u64 best = 0;
+    float low = __builtin_inff();
+    const RowSpace& w = s.space[row];
+    if ((int)threadIdx.x < s.chunks) best = w.best[threadIdx.x], low = w.low[threadIdx.x];
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const u64 o = __shfl_xor(best, off, 64);
+      best = o > best ? o : best;
+      low = fminf(low, __shfl_xor(low, off, 64));
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best, redf[threadIdx.x >> 6] = low;
+    __syncthreads();
+    for (int i = 0; i < kMaxChunks / 64; ++i) best = red[i] > best ? red[i] : best, low = fminf(low, redf[i]);
+    __syncthreads();
+    top_key = (uint32_t)(best >> 32);
+    top_index = (int)~(uint32_t)best;
+    top = logit_of_key(top_key);
+    temperature = s.a.temperature ? s.a.temperature[row] : 1.0f;
+    greedy = !(temperature > 0.0f) || top_key == 0xFFFFFFFFu || !(fabsf(top) <= 3.402823466e38f);
+    dtop = top, per_unit = 1.44269504088896340735992468100 / (double)temperature, unit_bits = s.unit_bits;
+    const float range = fminf(s.spread * temperature, top - low);
+    steps = fminf((float)(kBuckets - 2) / range, 1.0e30f);
   }
+  __device__ double weight(float v) const { return exp2_falling(((double)v - dtop) * per_unit, unit_bits); }  // unrounded
+  __device__ u64 fixed(float v) const { return rint_u64(weight(v)); }
+  // Falls with the logit; equal logits share a step.  The last step holds the logits without weight: -inf (also
+  // where inf * 0 is NaN) and what is further than 2047 / 2046 of the spread below the maximum.
+  __device__ int step(float v) const { return (int)fminf((top - v) * steps, (float)(kBuckets - 1)); }
+};
+
+template <class T>
+__device__ __forceinline__ const T* row_of(const SampleArgs& a, int row) {
+  return static_cast<const T*>(a.logits) + row * a.row_stride;
+}
+
+// f(logit, index) over a block's chunk of `per` tokens of a row, eight loads in flight a thread (N of them).
+template <int N, class T, class F>
+__device__ __forceinline__ void over_chunk(const T* x, int vocab, int per, F&& f) {
+  constexpr int kAhead = 8;
+  const int end = min(vocab, ((int)blockIdx.x + 1) * per);
+  for (int i0 = blockIdx.x * per + threadIdx.x; i0 < end; i0 += kAhead * N) {
+    float v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v[j] = logit_at(x, min(i0 + j * N, end - 1));
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j * N < end) f(v[j], i0 + j * N);
+  }
+}
+
+// grid = (chunks, rows).  Also clears the row's histogram.
+template <class T>
+__global__ void __launch_bounds__(kChunkThreads) sample_max_kernel(Sampler s) {
+  __shared__ u64 red[kChunkThreads / 64];
+  __shared__ float redf[kChunkThreads / 64];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  const T* x = row_of<T>(s.a, row);
+  RowSpace& w = s.space[row];
+  for (int i = blockIdx.x * kChunkThreads + tid; i < kBuckets; i += gridDim.x * kChunkThreads) w.weights[i] = 0, w.counts[i] = 0;
+  if (blockIdx.x == 0 && tid == 0) w.listed = 0;
+  u64 best = 0;
+  float low = __builtin_inff();
+  over_chunk<kChunkThreads>(x, s.a.vocab, s.per_chunk, [&](float v, int i) {
+    const u64 k = ((u64)order_key(v) << 32) | (u64)(~(uint32_t)i);
+    best = k > best ? k : best;
+    if (v > -__builtin_inff()) low = fminf(low, v);
+  });
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     const u64 o = __shfl_xor(best, off, 64);
     best = o > best ? o : best;
+    low = fminf(low, __shfl_xor(low, off, 64));
   }
-  if ((tid & 63) == 0) red[tid >> 6] = best;
+  if ((tid & 63) == 0) red[tid >> 6] = best, redf[tid >> 6] = low;
   __syncthreads();
-  for (int w = 0; w < kThreads / 64; ++w) best = red[w] > best ? red[w] : best;
-  const uint32_t top_key = (uint32_t)(best >> 32);
-  const float top = logit_of_key(top_key);
-  const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-  const bool finite = top_key != 0xFFFFFFFFu && fabsf(top) <= 3.402823466e38f;
-  if (!(temperature > 0.0f) || !finite) {
-    if (tid == 0) a.token_ids[row] = (int)~(uint32_t)best;
+  if (tid != 0) return;
+  for (int i = 1; i < kChunkThreads / 64; ++i) best = red[i] > best ? red[i] : best, low = fminf(low, redf[i]);
+  w.best[blockIdx.x] = best;
+  w.low[blockIdx.x] = low;
+}
+
+__device__ __forceinline__ bool wants_top_k(const Sampler& s, int row, int& k) {
+  k = s.a.top_k ? s.a.top_k[row] : 0;
+  return k > 0 && k < s.a.vocab;
+}
+__device__ __forceinline__ bool wants_top_p(const Sampler& s, int row, float& p) {
+  p = s.a.top_p ? s.a.top_p[row] : 1.0f;
+  return p < 1.0f;
+}
+
+// grid = (chunks, rows).
+template <class T>
+__global__ void __launch_bounds__(kHistThreads) sample_hist_kernel(Sampler s) {
+  __shared__ u64 weights[kBuckets];
+  __shared__ uint32_t counts[kBuckets];
+  __shared__ u64 red[kHistThreads / 64];
+  __shared__ float redf[kHistThreads / 64];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  int k;
+  float p;
+  const bool top_p = wants_top_p(s, row, p);
+  if (!wants_top_k(s, row, k) && !top_p) return;
+  const Row r(s, row, red, redf);
+  if (r.greedy) return;
+  for (int i = tid; i < kBuckets; i += kHistThreads) weights[i] = 0, counts[i] = 0;
+  __syncthreads();
+  const T* x = row_of<T>(s.a, row);
+  over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int) {
+    const int b = r.step(v);
+    atomicAdd(&counts[b], 1u);
+    if (top_p) {
+      const u64 n = r.fixed(v);
+      if (n) atomicAdd(&weights[b], n);
+    }
+  });
+  __syncthreads();
+  RowSpace& w = s.space[row];
+  for (int i = tid; i < kBuckets; i += kHistThreads) {
+    if (counts[i]) atomicAdd(&w.counts[i], counts[i]);
+    if (weights[i]) atomicAdd(&w.weights[i], weights[i]);
+  }
+}
+
+// The histogram of a row held by a block of N threads: thread t has kBuckets / N adjacent steps and what is before.
+template <int N>
+struct Held {
+  static constexpr int kPer = kBuckets / N;
+  u64 count[kPer], weight[kPer], count_before, weight_before, weight_total;
+  __device__ explicit Held(const RowSpace& w) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) count[i] = w.counts[kPer * threadIdx.x + i], weight[i] = w.weights[kPer * threadIdx.x + i];
+  }
+  __device__ void scan(u64* red) {
+    u64 n = 0, x = 0, none;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) n += count[i], x += weight[i];
+    count_before = block_scan<N>(n, red, none);
+    weight_before = block_scan<N>(x, red, weight_total);
+  }
+  struct Found {
+    int step;
+    u64 before;  // counts or weight before the step
+    u64 at, tokens, tokens_before;  // weight and tokens of the step
+  };
+  // The step in which a rank ends: the last one with tokens before which there are fewer than `limit` (by weight: the
+  // last one with weight before which there is less than `goal`).  Steps behind `last` do not count, and step
+  // `last` counts as `last_weight`.
+  __device__ Found find(bool by_weight, u64 limit, double goal, int last, u64 last_weight, u64* pick, uint32_t* pick_step) const {
+    if (threadIdx.x == 0) *pick_step = 0u;
+    __syncthreads();
+    u64 run = by_weight ? weight_before : count_before, n = count_before, before = 0, at = 0, tokens = 0, tokens_before = 0;
+    int mine = threadIdx.x == 0 ? 0 : -1;
+    if (threadIdx.x == 0) at = weight[0], tokens = count[0];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = kPer * threadIdx.x + i;
+      const u64 x = !by_weight ? count[i] : b < last ? weight[i] : b == last ? last_weight : 0ull;
+      if (x && (by_weight ? (double)run < goal : run < limit))
+        mine = b, before = run, at = weight[i], tokens = count[i], tokens_before = n;
+      run += by_weight ? weight[i] : x;
+      n += count[i];
+    }
+    if (mine >= 0) atomicMax(pick_step, (uint32_t)mine);
+    __syncthreads();
+    if (mine >= 0 && *pick_step == (uint32_t)mine) pick[0] = before, pick[1] = at, pick[2] = tokens, pick[3] = tokens_before;
+    __syncthreads();
+    const Found f{(int)*pick_step, pick[0], pick[1], pick[2], pick[3]};
+    __syncthreads();
+    return f;
+  }
+  // Weight before step b.
+  __device__ u64 weight_to(int b, u64* pick) const {
+    if (b >= kBuckets) return weight_total;
+    if (b / kPer == (int)threadIdx.x) {
+      u64 x = weight_before;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x += i < b % kPer ? weight[i] : 0ull;
+      pick[0] = x;
+    }
+    __syncthreads();
+    const u64 x = pick[0];
+    __syncthreads();
+    return x;
+  }
+};
+
+// The steps whose tokens decide the cuts of a row: that of top-k (-1: none, or among tokens without weight) and
+// those in which top-p can end, which depends on the part of the top-k step that is kept (empty: high < low).
+struct Needed {
+  int k_step, low, high;
+  u64 k_before;
+  bool listed;  // their tokens fit the list
+  __device__ bool has(int b) const { return b == k_step || (b >= low && b <= high); }
+};
+template <int N>
+__device__ Needed needed_steps(const Held<N>& h, bool top_k, int k, bool top_p, float p, u64* pick, uint32_t* pick_step) {
+  Needed n{-1, 0, -1, 0, false};
+  u64 at = 0, tokens = 0;
+  if (top_k) {
+    const auto f = h.find(false, (u64)k, 0.0, kBuckets, 0, pick, pick_step);
+    if (f.step < kBuckets - 1) n.k_step = f.step, n.k_before = f.before, at = f.at, tokens = f.tokens;
+  }
+  if (top_p) {
+    const int last = n.k_step < 0 ? kBuckets : n.k_step;
+    const u64 before = h.weight_to(last, pick);
+    const double least = (double)p * (double)before, most = (double)p * (double)(before + at);
+    if (most > 0.0) {
+      const auto hi = h.find(true, 0, most, last, at, pick, pick_step);
+      const auto lo = last == kBuckets ? hi : h.find(true, 0, least, last, at, pick, pick_step);
+      n.high = hi.step, n.low = lo.step;
+      tokens += hi.tokens_before + hi.tokens - lo.tokens_before;  // (the top-k step may count twice)
+    }
+  }
+  n.listed = tokens <= (u64)kList;
+  return n;
+}
+
+// Lists the keys of the needed steps' tokens; every block finds the steps for itself.  grid = (chunks, rows).
+template <class T>
+__global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
+  __shared__ u64 red[kHistThreads / 64], pick[4];
+  __shared__ float redf[kHistThreads / 64];
+  __shared__ uint32_t pick_step, found, at;
+  __shared__ uint32_t keys[kList];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  int k;
+  float p;
+  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
+  if (!top_k && !top_p) return;
+  RowSpace& w = s.space[row];
+  Held<kHistThreads> held(w);
+  const Row r(s, row, red, redf);
+  if (r.greedy) return;
+  held.scan(red);
+  if (tid == 0) found = 0u;
+  const Needed need = needed_steps(held, top_k, k, top_p, p, pick, &pick_step);
+  if (blockIdx.x == 0 && tid == 0) {
+    w.k_step = need.k_step, w.p_low = need.low, w.p_high = need.high, w.k_before = need.k_before;
+    if (!need.listed) w.listed = kUnlisted;
+  }
+  if (!need.listed) return;
+  const T* x = row_of<T>(s.a, row);
+  over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int) {
+    if (need.has(r.step(v))) keys[atomicAdd(&found, 1u)] = order_key(v);
+  });
+  __syncthreads();
+  if (tid == 0 && found) at = atomicAdd(&w.listed, found);  // one a block: they are serialized over the row
+  __syncthreads();
+  for (int i = tid; i < (int)found; i += kHistThreads) w.list[at + i] = keys[i];
+}
+
+// The cuts of one row: grid = rows.
+template <class T>
+__global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
+  __shared__ u64 hist[kBuckets];
+  __shared__ uint32_t count[kBuckets];
+  __shared__ uint32_t list[kList];
+  __shared__ u64 red[kChunkThreads / 64], pick[4];
+  __shared__ float redf[kChunkThreads / 64];
+  __shared__ uint32_t pick_step, differ, sample_key;
+  const int row = blockIdx.x, tid = threadIdx.x, vocab = s.a.vocab;
+  Cut cut{0u, 0u};  // everything: every key is above 0 (-inf has key 0x007FFFFF)
+  int k;
+  float p;
+  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
+  RowSpace& w = s.space[row];
+  if (!top_k && !top_p) {
+    if (tid == 0) w.cut = cut;
     return;
   }
-  const double dtop = top, dtemp = temperature;
-  const float qmin = a.min_p ? a.min_p[row] : 0.0f;
-  const double least = qmin > 0.0f ? (double)fminf(qmin, 1.0f) : 0.0;
-  auto real_weight = [&](float v) { return exp(((double)v - dtop) / dtemp); };
-  auto fixed = [&](double w) { return (u64)rint(w * unit); };
+  Held<kChunkThreads> held(w);
+  const uint32_t listed = w.listed;
+  Needed need{w.k_step, w.p_low, w.p_high, w.k_before, listed != kUnlisted};
+  if (need.listed)
+    for (int i = tid; i < (int)listed; i += kChunkThreads) list[i] = w.list[i];
+  const Row r(s, row, red, redf);
+  if (r.greedy) return;  // (no later launch reads its cut)
+  const T* x = row_of<T>(s.a, row);
+  held.scan(red);
 
-  // The (T, n) of a rank by counts (`by_weight` false: the first `k` tokens) or by weight within `in` (tokens
-  // before which the weight is below `goal`).  One histogram per radix step, scanned from the largest bucket.
-  auto select = [&](bool by_weight, uint32_t k, double goal, Cut in) {
-    uint32_t prefix = 0, above_n = 0;
-    u64 above = 0;
-    for (int step = 0; step < 3; ++step) {
-      const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
-      for (int i = tid; i < kBuckets; i += kThreads) hist[i] = 0, count[i] = 0;
+  // The (T, n) of a rank among the listed tokens of one step (`above` in front of them) or the whole row (step < 0), by
+  // counts (the first `limit`) or by weight within `in` (tokens before which the weight is below `goal`): radix steps
+  // of up to 11 bits of the key from the highest bit in which the candidates differ, each a histogram scanned
+  // from its largest bucket, until the candidates are equal.
+  auto select = [&](int step, u64 above, bool by_weight, u64 limit, double goal, Cut in) {
+    const int n = step < 0 ? vocab : (int)listed;
+    int known = 32;  // candidates: key >> known == prefix
+    uint32_t prefix = 0;
+    auto candidate = [&](int i, uint32_t& key) {
+      key = step < 0 ? order_key(logit_at(x, i)) : list[i];
+      if (known < 32 && (key >> known) != prefix) return false;
+      if (by_weight && key <= in.key) return false;
+      return step < 0 || r.step(logit_of_key(key)) == step;
+    };
+    const bool extra = by_weight && in.ties != 0;  // the cut's own tokens count as in.ties of them
+    for (;;) {
+      for (int i = tid; i < kBuckets; i += kChunkThreads) hist[i] = 0, count[i] = 0;
+      if (tid == 0) differ = 0u, sample_key = 0u, pick_step = 0xFFFFFFFFu;
       __syncthreads();
-      for (int i = tid; i < vocab; i += kThreads) {
-        const float v = logit_at(x, i);
-        const uint32_t key = order_key(v);
-        if (step > 0 && (key >> (shift + bits)) != prefix) continue;
-        if (by_weight && key <= in.key) continue;
-        const uint32_t bucket = (key >> shift) & ((1u << bits) - 1u);
+      const bool extra_now = extra && (known == 32 || (in.key >> known) == prefix);
+      uint32_t key, mine = 0, lo = 0xFFFFFFFFu;
+      for (int i = tid; i < n; i += kChunkThreads)
+        if (candidate(i, key)) mine = max(mine, key), lo = min(lo, key);
+      if (extra_now && tid == 0) mine = max(mine, in.key), lo = min(lo, in.key);
+      if (mine) atomicMax(&sample_key, mine);
+      __syncthreads();
+      const uint32_t top = sample_key;  // the largest candidate
+      if (top == 0u) return in;
+      if (mine && (lo ^ top) != 0u) atomicMax(&differ, lo ^ top);  // its highest bit: the highest that differs
+      __syncthreads();
+      const uint32_t bits_off = differ;
+      const int hb = bits_off ? 31 - __clz((int)bits_off) : -1, shift = max(0, hb - 10), bits = hb + 1 - shift;
+      const uint32_t mask = bits ? (1u << bits) - 1u : 0u;
+      for (int i = tid; i < n; i += kChunkThreads) {
+        if (!candidate(i, key)) continue;
+        const uint32_t bucket = (key >> shift) & mask;
         atomicAdd(&count[bucket], 1u);
-        if (by_weight) atomicAdd(&hist[bucket], fixed(real_weight(v)));
+        if (by_weight) atomicAdd(&hist[bucket], r.fixed(logit_of_key(key)));
       }
       __syncthreads();
-      if (by_weight && tid == 0 && in.ties && (step == 0 || (in.key >> (shift + bits)) == prefix)) {
-        const uint32_t bucket = (in.key >> shift) & ((1u << bits) - 1u);
+      if (extra_now && tid == 0) {
+        const uint32_t bucket = (in.key >> shift) & mask;
         count[bucket] += in.ties;
-        hist[bucket] += in.ties * fixed(real_weight(logit_of_key(in.key)));
+        hist[bucket] += in.ties * r.fixed(logit_of_key(in.key));
       }
       __syncthreads();
-      const int hi = kBuckets - 1 - 2 * tid, lo = hi - 1;  // this thread's two buckets, the largest first
-      u64 total, none;
-      const u64 n_before = block_scan((u64)count[hi] + count[lo], red, total);
-      const u64 w_before = by_weight ? block_scan(hist[hi] + hist[lo], red, none) : 0;
-      if (tid == 0) pick_bucket = 0xFFFFFFFFu;
-      __syncthreads();
-      // the last bucket that holds a token of the rank: those before it hold fewer than asked for
-      u64 n = above_n + n_before, w = above + w_before;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int bucket = j ? lo : hi;
-        const u64 n_next = n + count[bucket], w_next = w + hist[bucket];
-        const bool starts = by_weight ? hist[bucket] && (double)w < goal : count[bucket] && n < k;
-        const bool ends = by_weight ? !((double)w_next < goal) : n_next >= k;
-        if (starts && ends) pick_bucket = bucket, pick_above = w, pick_count_above = (uint32_t)n;
-        n = n_next, w = w_next;
-      }
-      __syncthreads();
-      if (pick_bucket == 0xFFFFFFFFu) return in;  // everything is kept
-      prefix = (prefix << bits) | pick_bucket;
-      above = pick_above;
-      above_n = pick_count_above;
-      const uint32_t held = count[pick_bucket];
-      __syncthreads();
-      if (step == 2) {
-        Cut c{prefix, 0};
+      if (hb < 0) {  // all equal (bucket 0)
+        const u64 have = count[0];
+        Cut c{top, 0};
         if (!by_weight) {
-          c.ties = k - above_n;
+          c.ties = (uint32_t)min(have, limit - above);
         } else {
-          const u64 w1 = fixed(real_weight(logit_of_key(prefix)));
-          uint32_t j = 1;  // the first tie has less than `goal` before it
-          const double guess = (goal - (double)above) / (double)w1;
-          if (guess > 2.0) j = guess < (double)held ? (uint32_t)guess - 1u : held;
-          while (j > 1 && !((double)(above + (u64)(j - 1) * w1) < goal)) --j;
-          while (j < held && (double)(above + (u64)j * w1) < goal) ++j;
-          c.ties = j;
+          const u64 one = r.fixed(logit_of_key(top));
+          u64 j = 1;  // the first tie has less than `goal` before it
+          const double guess = (goal - (double)above) / (double)one;
+          if (guess > 2.0) j = guess < (double)have ? (u64)guess - 1u : have;
+          while (j > 1 && !((double)(above + (j - 1) * one) < goal)) --j;
+          while (j < have && (double)(above + j * one) < goal) ++j;
+          c.ties = (uint32_t)j;
         }
         return c;
       }
+      // this thread's adjacent buckets, the largest first; the smallest non-empty one that starts within the rank
+      constexpr int kPer = kBuckets / kChunkThreads;
+      const int hi = kBuckets - 1 - kPer * tid;
+      u64 b[kPer], sum = 0, total, my_before = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) b[i] = by_weight ? hist[hi - i] : count[hi - i], sum += b[i];
+      u64 run = above + block_scan<kChunkThreads>(sum, red, total);
+      uint32_t my = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (b[i] && (by_weight ? (double)run < goal : run < limit)) my = hi - i, my_before = run;
+        run += b[i];
+      }
+      if (my != 0xFFFFFFFFu) atomicMin(&pick_step, my);
+      __syncthreads();
+      const uint32_t got = pick_step;
+      if (got == 0xFFFFFFFFu) return in;
+      if (got == my) pick[0] = my_before;
+      __syncthreads();
+      above = pick[0];
+      prefix = shift + bits < 32 ? ((top >> (shift + bits)) << bits) | got : got;
+      known = shift;
+      __syncthreads();
     }
-    return in;
   };
 
-  Cut cut{0u, 0u};  // every key is above 0 (-inf has key 0x007FFFFF)
-  const int k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && k < vocab) cut = select(false, (uint32_t)k, 0.0, cut);
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  if (p < 1.0f) {
-    // total weight of what is kept so far
-    u64 sum = 0, total;
-    for (int i = tid; i < vocab; i += kThreads) {
-      const float v = logit_at(x, i);
-      if (order_key(v) > cut.key) sum += fixed(real_weight(v));
+  if (need.k_step >= 0)
+    cut = need.listed ? select(need.k_step, need.k_before, false, (u64)k, 0.0, cut) : select(-1, 0, false, (u64)k, 0.0, cut);
+  if (top_p) {
+    // weight of what is kept so far: whole steps, and the kept part of the cut one
+    const int last = need.k_step < 0 ? kBuckets : need.k_step;
+    u64 total = held.weight_to(last, pick), last_weight = 0;
+    if (need.k_step >= 0) {
+      u64 part = 0;
+      const int n = need.listed ? (int)listed : vocab;
+      for (int i = tid; i < n; i += kChunkThreads) {
+        const uint32_t key = need.listed ? list[i] : order_key(logit_at(x, i));
+        const float v = logit_of_key(key);
+        if (key > cut.key && r.step(v) == last) part += r.fixed(v);
+      }
+      if (tid == 0) part += cut.ties * r.fixed(logit_of_key(cut.key));
+      block_scan<kChunkThreads>(part, red, last_weight);
     }
-    block_scan(sum, red, total);
-    if (cut.ties) total += cut.ties * fixed(real_weight(logit_of_key(cut.key)));
+    total += last_weight;
     const double goal = (double)p * (double)total;
-    cut = goal > 0.0 ? select(true, 0, goal, cut) : Cut{top_key, 1u};
+    if (!(goal > 0.0)) {
+      cut = Cut{r.top_key, 1u};
+    } else if (!need.listed) {
+      cut = select(-1, 0, true, 0, goal, cut);
+    } else {
+      const auto f = held.find(true, 0, goal, last, last_weight, pick, &pick_step);
+      cut = select(f.step, f.before, true, 0, goal, f.step == last ? cut : Cut{0u, 0u});
+    }
   }
+  if (tid == 0) w.cut = cut;
+}
 
-  // Draw: weights and ties of index ranges, the range that holds the goal, then the token in it
-  const int per = ((vocab + kSegments - 1) / kSegments + 63) / 64 * 64;  // tokens of a range: whole waves
-  const int segments = (vocab + per - 1) / per;
-  u64* seg_w = hist;
-  uint32_t* seg_n = count;
-  const int wave = tid >> 6, lane = tid & 63;
-  auto kept_weight = [&](float v) {
-    const double w = real_weight(v);
-    return w >= least ? fixed(w) : 0ull;
-  };
-  __syncthreads();
-  for (int s = wave; s < segments; s += kThreads / 64) {
+// The kept weight of a logit, without regard to ties.
+__device__ __forceinline__ u64 kept_weight(const Row& r, float v, double least) {
+  const double w = r.weight(v);
+  return w >= least ? rint_u64(w) : 0ull;
+}
+__device__ __forceinline__ double least_weight(const Sampler& s, int row) {
+  const float q = s.a.min_p ? s.a.min_p[row] : 0.0f;
+  return q > 0.0f ? (double)fminf(q, 1.0f) * (double)(1ull << s.unit_bits) : 0.0;
+}
+
+// Kept weight above the cut, and number of tokens at it, of each segment: a wave per segment, in turn.
+// grid = (blocks, rows).
+template <class T>
+__global__ void __launch_bounds__(kChunkThreads) sample_segment_kernel(Sampler s) {
+  __shared__ u64 red[kChunkThreads / 64];
+  __shared__ float redf[kChunkThreads / 64];
+  const int row = blockIdx.y, lane = threadIdx.x & 63;
+  const T* x = row_of<T>(s.a, row);
+  const Cut cut = s.space[row].cut;
+  const double least = least_weight(s, row);
+  const Row r(s, row, red, redf);
+  if (r.greedy) return;
+  for (int seg = blockIdx.x * (kChunkThreads / 64) + (threadIdx.x >> 6); seg < s.segments; seg += gridDim.x * (kChunkThreads / 64)) {
     u64 w = 0;
     uint32_t n = 0;
-    for (int i = s * per + lane; i < min(vocab, (s + 1) * per); i += 64) {
-      const float v = logit_at(x, i);
-      const uint32_t key = order_key(v);
-      if (key > cut.key) w += kept_weight(v);
-      if (key == cut.key) ++n;
+    for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
+      const int i0 = (seg * s.blocks_per_segment + blk) * kSegment + lane;
+      float v[kSegment / 64];
+#pragma unroll
+      for (int j = 0; j < kSegment / 64; ++j) v[j] = i0 + 64 * j < s.a.vocab ? logit_at(x, i0 + 64 * j) : -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < kSegment / 64; ++j) {
+        const uint32_t key = order_key(v[j]);
+        if (key > cut.key) w += kept_weight(r, v[j], least);
+        if (key == cut.key && i0 + 64 * j < s.a.vocab) ++n;
+      }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
       w += __shfl_xor(w, off, 64);
       n += __shfl_xor(n, off, 64);
     }
-    if (lane == 0) seg_w[s] = w, seg_n[s] = n;
+    if (lane == 0) {
+      s.seg_weight[(size_t)row * s.segments + seg] = w;
+      s.seg_ties[(size_t)row * s.segments + seg] = n;
+    }
   }
+}
+
+// The draw: the segment that holds the goal, then the token in it.  One segment a thread; grid = rows.
+template <class T>
+__global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
+  __shared__ u64 red[kThreads / 64];
+  __shared__ float redf[kThreads / 64];
+  __shared__ u64 pick_above;
+  __shared__ uint32_t pick_segment, pick_seen;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  // everything that the row's weights do not decide, before the first wait
+  const bool live = tid < s.segments;
+  const u64 my_weight = live ? s.seg_weight[(size_t)row * s.segments + tid] : 0ull;
+  const u64 my_ties = live ? s.seg_ties[(size_t)row * s.segments + tid] : 0ull;
+  const Cut cut = s.space[row].cut;
+  const double least = least_weight(s, row);
+  const float uf = s.a.uniforms[row];
+  const Row r(s, row, red, redf);
+  if (r.greedy) {
+    if (tid == 0) s.a.token_ids[row] = r.top_index;
+    return;
+  }
+  const u64 tie = cut.ties ? kept_weight(r, logit_of_key(cut.key), least) : 0ull;
+  u64 none, total;
+  const u64 seen = block_scan<kThreads>(my_ties, red, none);
+  const u64 kept = seen >= cut.ties ? 0ull : min(my_ties, (u64)cut.ties - seen);
+  const u64 weight = my_weight + kept * tie;
+  const u64 before = block_scan<kThreads>(weight, red, total);
+  const double goal = (uf > 0.0f ? (double)fminf(uf, 1.0f) : 0.0) * (double)total;
+  // the last segment with kept weight that starts at or below the goal
+  const bool within = weight && !((double)before > goal);
+  if (tid == 0) pick_segment = 0u;
   __syncthreads();
-  const u64 tie_w = cut.ties ? kept_weight(logit_of_key(cut.key)) : 0ull;
-  const u64 n_mine = tid < segments ? seg_n[tid] : 0u;
-  u64 n_all, total;
-  const u64 n_before = block_scan(n_mine, red, n_all);
-  const u64 ties_mine = n_before >= cut.ties ? 0ull : min(n_mine, (u64)cut.ties - n_before);
-  const u64 w_mine = tid < segments ? seg_w[tid] + ties_mine * tie_w : 0ull;
-  const u64 w_before = block_scan(w_mine, red, total);
-  const float uf = a.uniforms[row];
-  const double u = uf > 0.0f ? (double)fminf(uf, 1.0f) : 0.0;
-  const double goal = u * (double)total;
-  // the first token whose running sum exceeds goal; where rounding leaves none, the last one kept
-  if (tid == 0) pick_bucket = 0u;
+  if (within) atomicMax(&pick_segment, (uint32_t)tid);
   __syncthreads();
-  if (w_mine && !((double)w_before > goal)) atomicMax(&pick_bucket, (uint32_t)tid);
+  if (tid == (int)pick_segment) pick_above = before, pick_seen = (uint32_t)seen;
   __syncthreads();
-  if ((uint32_t)tid == pick_bucket) pick_above = w_before, pick_count_above = (uint32_t)n_before;
-  __syncthreads();
-  if (wave != 0) return;
-  const int s = pick_bucket;
-  u64 run = pick_above;
-  uint32_t seen = pick_count_above;
+  if (tid >= 64) return;
+  // one wave: each lane eight adjacent tokens
+  constexpr int kLane = kSegment / 64;
+  const T* x = row_of<T>(s.a, row);
+  u64 above = pick_above;
+  uint32_t rank0 = pick_seen;
   int token = 0;
-  for (int i0 = s * per; i0 < min(vocab, (s + 1) * per); i0 += 64) {
-    const int i = i0 + lane;
-    const float v = i < vocab ? logit_at(x, i) : 0.0f;
-    const uint32_t key = i < vocab ? order_key(v) : 0u;
-    const bool tie = i < vocab && key == cut.key;
-    const u64 ties = __ballot(tie);
-    const uint32_t rank = seen + __popcll(ties & ((1ull << lane) - 1ull));
-    u64 w = key > cut.key ? kept_weight(v) : 0ull;
-    if (tie && rank < cut.ties) w = tie_w;
-    u64 inc = w;
+  for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
+    const int first = ((int)pick_segment * s.blocks_per_segment + blk) * kSegment + kLane * tid;
+    float v[kLane];
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) v[j] = first + j < s.a.vocab ? logit_at(x, first + j) : -__builtin_inff();
+    uint32_t held = 0;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) held += first + j < s.a.vocab && order_key(v[j]) == cut.key ? 1u : 0u;
+    uint32_t rank = held;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const u64 o = __shfl_up(inc, off, 64);
-      if (lane >= off) inc += o;
+      const uint32_t o = __shfl_up(rank, off, 64);
+      if (tid >= off) rank += o;
     }
-    const u64 past = __ballot(w && (double)(run + inc) > goal), some = __ballot(w != 0);
-    if (some) token = i0 + 63 - __clzll(some);
-    if (past) {
-      token = i0 + __ffsll((unsigned long long)past) - 1;
-      break;
+    const uint32_t rank_next = rank0 + __shfl(rank, 63, 64);
+    rank += rank0 - held;
+    u64 here[kLane], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      const uint32_t key = order_key(v[j]);
+      here[j] = key > cut.key ? kept_weight(r, v[j], least) : 0ull;
+      if (first + j < s.a.vocab && key == cut.key && rank++ < cut.ties) here[j] = tie;
+      sum += here[j];
     }
-    run += __shfl(inc, 63, 64);
-    seen += __popcll(ties);
+    u64 run = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const u64 o = __shfl_up(run, off, 64);
+      if (tid >= off) run += o;
+    }
+    const u64 above_next = above + __shfl(run, 63, 64);
+    run += above - sum;
+    int past = -1, some = -1;  // the lane's first token beyond the goal, and its last one with weight
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+      run += here[j];
+      if (here[j]) {
+        some = j;
+        if (past < 0 && (double)run > goal) past = j;
+      }
+    }
+    const u64 beyond = __ballot(past >= 0), any = __ballot(some >= 0);
+    if (any) {
+      const int lane = beyond ? __ffsll(beyond) - 1 : 63 - __clzll(any);
+      token = __shfl(first + (beyond ? past : some), lane, 64);
+    }
+    if (beyond) break;
+    above = above_next;
+    rank0 = rank_next;
   }
-  if (lane == 0) a.token_ids[row] = token;
+  if (tid == 0) s.a.token_ids[row] = token;
+}
+
+template <class T>
+void run_sample(const Sampler& s, hipStream_t st) {
+  const int rows = s.a.rows;
+  const int segment_blocks = (s.segments + 3) / 4;
+  hipLaunchKernelGGL(sample_max_kernel<T>, dim3(s.chunks, rows), dim3(kChunkThreads), 0, st, s);
+  if (s.a.top_k || s.a.top_p) {
+    hipLaunchKernelGGL(sample_hist_kernel<T>, dim3(s.hist_chunks, rows), dim3(kHistThreads), 0, st, s);
+    hipLaunchKernelGGL(sample_list_kernel<T>, dim3(s.hist_chunks, rows), dim3(kHistThreads), 0, st, s);
+  }
+  hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(rows), dim3(kChunkThreads), 0, st, s);
+  hipLaunchKernelGGL(sample_segment_kernel<T>, dim3(segment_blocks, rows), dim3(kChunkThreads), 0, st, s);
+  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(rows), dim3(kThreads), 0, st, s);
 }
 
 }  // namespace
 
-size_t sample_workspace_bytes(int, int) { return 0; }
+static int blocks_per_segment(int vocab) { return (vocab + kThreads * kSegment - 1) / (kThreads * kSegment); }
+static int segments_of(int vocab) {
+  const int tokens = blocks_per_segment(vocab) * kSegment;
+  return (vocab + tokens - 1) / tokens;
+}
 
-void launch_sample(const SampleArgs& a, void*, hipStream_t st) {
-  // weights of up to 2^24 tokens sum to less than 2^62
-  int bits = 0;
+size_t sample_workspace_bytes(int rows, int vocab) {
+  return (size_t)rows * (sizeof(RowSpace) + segments_of(vocab) * (sizeof(u64) + sizeof(uint32_t)));
+}
+
+void launch_sample(const SampleArgs& a, void* workspace, hipStream_t st) {
+  Sampler s{};
+  s.a = a;
+  int bits = 0;  // weights of up to 2^24 tokens sum to less than 2^62
   while ((1 << bits) < a.vocab) ++bits;
-  const double unit = (double)(1ull << (62 - bits));
+  s.unit_bits = 62 - bits < 50 ? 62 - bits : 50;
+  s.spread = (float)(s.unit_bits + 1) * 0.6931472f;
+  auto split = [&](int blocks, int least, int threads, int& chunks, int& per) {
+    chunks = blocks / a.rows;
+    const int most = (a.vocab + least - 1) / least;
+    chunks = chunks > most ? most : chunks;
+    chunks = chunks < 1 ? 1 : chunks > kMaxChunks ? kMaxChunks : chunks;
+    per = ((a.vocab + chunks - 1) / chunks + threads - 1) / threads * threads;
+    chunks = (a.vocab + per - 1) / per;
+  };
+  split(1024, 1024, kChunkThreads, s.chunks, s.per_chunk);  // about four a CU over all rows, of 1024 tokens at least
+  // histogram and list: two of 512 threads a CU (64 rows of 151936: 22 + 19 us; 256 x 1024 threads 22 + 18 but one row
+  // 7 + 12 instead of 6 + 9 us; 1024 blocks of 256 threads 23 + 19 and 8 + 9; 512 of 1024 26 + 29)
+  split(512, 4 * kHistThreads, kHistThreads, s.hist_chunks, s.hist_per_chunk);
+  s.segments = segments_of(a.vocab);
+  s.blocks_per_segment = blocks_per_segment(a.vocab);
+  s.space = static_cast<RowSpace*>(workspace);
+  s.seg_weight = reinterpret_cast<u64*>(s.space + a.rows);
+  s.seg_ties = reinterpret_cast<uint32_t*>(s.seg_weight + (size_t)a.rows * s.segments);
   if (a.type == QWEN_TYPE_F32)
-    hipLaunchKernelGGL(sample_kernel<float>, dim3(a.rows), dim3(kThreads), 0, st, a, unit);
+    run_sample<float>(s, st);
   else
-    hipLaunchKernelGGL(sample_kernel<uint16_t>, dim3(a.rows), dim3(kThreads), 0, st, a, unit);
+    run_sample<uint16_t>(s, st);
 }
 
 }  // namespace qwen

@@ -20,7 +20,7 @@ int bad(const char* why) {
 }
 
 const char* size_problem(int rows, int vocab) {
-  if (rows < 1 || rows > (1 << 20)) return "sampling takes 1 .. 2^20 rows";
+  if (rows < 1 || rows > 65535) return "sampling takes 1 .. 65535 rows";  // (grid y)
   if (vocab < 1 || vocab > kSampleMaxVocab) return "sampling takes 1 .. 2^24 tokens";
   return nullptr;
 }
