@@ -91,9 +91,10 @@ def tolerance(dtype: str, dim: int, slack: np.ndarray, floor: np.ndarray, reach:
     2^-24 relative to sum |q k| (reach), of a query known to 2^-22 of its largest element (two fp16 terms; one
     holds a bf16 query); four further fp32 roundings of the scaled score and exp2's ulp.  A probability enters
     with a relative error of 2^-22 (two terms) or 2^-11 (one) as long as fp16 holds it as a normal number; the
-    largest probability enters as up to 2^15, and fp16's last place is never below 2^-24, so the rounding of a
-    far smaller one is at most 2^-25 / 2^15 = 2^-40 of the largest (floor).  An error e of every probability moves the output
+    largest probability enters as 2^15, or, in tiles of many rows, as 2^11 to 2^15 times the block's V scale over
+    the accumulator's unit (2^-6 to 1); fp16's last place is never below 2^-24, so the rounding of a far smaller
+    one is at most 2^-25 / 2^11 = 2^-36 of the largest (floor, in units of up to 2^6 |v|).  An error e of every probability moves the output
     by at most 2 e sum p |v|; the sums over the keys are fp32.  bf16 results are rounded by 2^-8 at most."""
     score = reach * ((dim + 8) * 2.0 ** -24 + 2.0 ** -21)
     p = score + (2.0 ** -20 if dtype == "f32" else 2.0 ** -11)
-    return 2 * p[..., None] * slack + 2.0 ** -40 * floor + (2.0 ** -22 if dtype == "f32" else 2.0 ** -8) * np.abs(out) + 1e-30
+    return 2 * p[..., None] * slack + 2.0 ** -30 * floor + (2.0 ** -22 if dtype == "f32" else 2.0 ** -8) * np.abs(out) + 1e-30

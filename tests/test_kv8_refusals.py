@@ -66,8 +66,9 @@ def test_kv8_refuses_overlapping_results(lib, op, which, over):
 
 @pytest.mark.parametrize("bad", [dict(heads=0), dict(heads=3), dict(heads=130), dict(heads=-2), dict(max_keys=0),
                                  dict(max_keys=513), dict(max_keys=-1), dict(scale=float("nan")),
-                                 dict(scale=float("inf")), dict(max_keys=512, ws=None), dict(max_keys=512, ws_bytes=16),
-                                 dict(max_keys=512, ws=PTR + 4)])
+                                 dict(scale=float("inf")), dict(c=cache(blocks=64), max_keys=4096, ws=None),
+                                 dict(c=cache(blocks=64), max_keys=4096, ws_bytes=16),
+                                 dict(c=cache(blocks=64), max_keys=4096, ws=PTR + 4)])
 def test_kv8_attention_refuses(lib, bad):
     assert call(lib, "attend", **bad) == 1
 

@@ -4,55 +4,11 @@
 // are applied to the products: no rounding beside the code's own.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
-#include "kernels.hpp"
-#include "qwen_device_math.hpp"
+#include "kv8_device.hpp"
 
 namespace qwen {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 namespace {
-
-struct Bf16 {  // storage of a bf16 element
-  uint16_t bits;
-};
-
-__device__ __forceinline__ float f32_nan() { return bits_f32(0x7FC00000u); }
-
-// Eight consecutive elements of a 16-byte aligned row.
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const Bf16* p, float (&x)[8]) {
-  const uint4 q = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[2 * i] = bits_f32(w[i] << 16), x[2 * i + 1] = bits_f32(w[i] & 0xFFFF0000u);
-}
-// Round to nearest even; NaN stays a quiet NaN.
-__device__ __forceinline__ uint32_t bf16_of(float x) {
-  const uint32_t b = f32_bits(x);
-  return (b & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC0u : (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
-}
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void store8(Bf16* p, const float (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = bf16_of(x[2 * i]) | (bf16_of(x[2 * i + 1]) << 16);
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void store4(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
-__device__ __forceinline__ void store4(Bf16* p, const f32x4& x) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(bf16_of(x[0]) | (bf16_of(x[1]) << 16), bf16_of(x[2]) | (bf16_of(x[3]) << 16));
-}
 
 // 4 x 4 bytes transposed: byte i of o[j] = byte j of w[i].
 __device__ __forceinline__ void transpose4(const uint32_t (&w)[4], uint32_t (&o)[4]) {
@@ -256,34 +212,19 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv
 }
 
 // ---- attention ------------------------------------------------------------------------------
-struct Kv8AttnArgs {
-  qwen_kv8_cache c;
-  qwen_kv8_rows q, out;
-  const int* positions;
-  int group, rows, max_keys;
-  float scale_log2e;
-  int nsplit, per_split;  // key splits of `per_split` blocks
-  float* part;            // [batch][kv_heads][rows * group][nsplit][D], nsplit > 1
-  float2* pml;            // [batch][kv_heads][rows * group][nsplit]
-};
-
-// Eight codes as fp16: 0x64uu is 1024 + uu, uu = code + 128.
-__device__ __forceinline__ half8 codes_to_half(uint32_t lo, uint32_t hi) {
-  const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
-  const uint32_t w[4] = {
-      __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u),
-      __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)};
-  half8 r;
-  __builtin_memcpy(&r, w, 16);
-  return r - (_Float16)1152.0f;
-}
-
 // The value of the lane whose column differs by 8 (row_ror:8).
 __device__ __forceinline__ float other_half(float x) {
   return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), 0x128, 0xF, 0xF, false));
 }
 
 constexpr float kProbBits = 15.0f;  // probabilities times 2^15: fp16 holds them normal down to 2^-29 of the largest
+
+// 16 bytes of the cache that nothing else reads (64 x 4096 fp32: 26.0 us, with cached loads 25.3 to 28.7).
+__device__ __forceinline__ uint4 load_once(const int8_t* p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
 
 // Attention of CT tiles of 16 query columns over one split of the keys.  Per wave and 64-token block:
 //   S^T = K Q^T (16x16x32 fp16, A = the codes of 16 tokens as they lie in the cache, B = query columns), so a lane
@@ -363,12 +304,12 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int s = 0; s < kHalves; ++s) kr[t][s] = *reinterpret_cast<const uint4*>(p + (s * kKv8Block + 16 * t) * 64);
+      for (int s = 0; s < kHalves; ++s) kr[t][s] = load_once(p + (s * kKv8Block + 16 * t) * 64);
   };
   auto load_v = [&](int blk) {
     const int8_t* p = a.c.v + (head0 + (size_t)blk * a.c.kv_heads) * block_bytes + col * 64 + 16 * g;
 #pragma unroll
-    for (int dt = 0; dt < kDimTiles; ++dt) vr[dt] = *reinterpret_cast<const uint4*>(p + dt * 16 * kKv8Block);
+    for (int dt = 0; dt < kDimTiles; ++dt) vr[dt] = load_once(p + dt * 16 * kKv8Block);
   };
   int blk = blk0 + wave;
   float sk = 0.0f, sv = 0.0f;
@@ -521,49 +462,72 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
   }
 }
 
-// Joins the key splits of one query row: grid = (rows * group, kv_heads, batch), block = D.
-template <class T, int D, int RT>
-__global__ void __launch_bounds__(D) kv8_merge_kernel(Kv8AttnArgs a) {
-  const int row = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, R = a.rows * a.group;
+// Joins the key splits of a query row: D / 4 lanes hold four dimensions each.  With many splits a block has one row
+// and divides the splits over its lane groups; with few it has a row per lane group.
+// grid = (rows * group / rows of a block, kv_heads, batch), block = 256.
+template <class T, int D, bool kMany>
+__global__ void __launch_bounds__(256) kv8_merge_kernel(Kv8AttnArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int row = kMany ? blockIdx.x : blockIdx.x * kGroups + grp, kvh = blockIdx.y, b = blockIdx.z, R = a.rows * a.group;
+  if (!kMany && row >= R) return;
   const int pos = a.positions[b];
-  // live splits: those of the row's tile group (RT rows), as kv8_attn_kernel counts them
-  const int i_last = min(R - 1, row / RT * RT + RT - 1) / a.group;
+  // live splits: those of the row's tile group, as the kernel before counts them
+  const int i_last = min(R - 1, row / a.tile_rows * a.tile_rows + a.tile_rows - 1) / a.group;
   const int kmax = pos < 0 ? 0 : (int)min((long long)pos + i_last + 1, (long long)a.max_keys);
   const int live = ((kmax + kKv8Block - 1) / kKv8Block + a.per_split - 1) / a.per_split;
   const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit;
-  float mm = -__builtin_inff();
-  for (int s = 0; s < live; ++s) mm = fmaxf(mm, a.pml[at + s].x);
-  float sum = 0.0f, o = 0.0f;
-  for (int s = 0; s < live; ++s) {
+  const f32x4* part = reinterpret_cast<const f32x4*>(a.part + at * D) + lane;
+  float m = -__builtin_inff(), sum = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = kMany ? grp : 0; s < live; s += kMany ? kGroups : 1) {
     const float2 v = a.pml[at + s];
-    const float f = v.x == -__builtin_inff() ? 1.0f : exp2f(v.x - mm);
-    sum += v.y * f;
-    o = fmaf(a.part[(at + s) * D + threadIdx.x], f, o);
+    const f32x4 x = part[(size_t)s * kLanes];
+    // (a split without keys for this row: maximum -inf, sum 0; a sum of NaN stays one)
+    const float mn = fmaxf(m, v.x), f0 = m == mn ? 1.0f : exp2f(m - mn), f1 = v.x == mn || v.x == -__builtin_inff() ? 1.0f : exp2f(v.x - mn);
+    sum = sum * f0 + v.y * f1;
+    o = o * f0 + x * f1;
+    m = mn;
   }
-  const float y = sum == 0.0f ? 0.0f : o * (1.0f / sum);
+  if constexpr (kMany) {
+    __shared__ float2 ml[kGroups];
+    __shared__ f32x4 os[kGroups][kLanes];
+    if (lane == 0) ml[grp] = make_float2(m, sum);
+    os[grp][lane] = o;
+    __syncthreads();
+    if (grp != 0) return;
+    float mm = m;
+    for (int g = 1; g < kGroups; ++g) mm = fmaxf(mm, ml[g].x);
+    sum = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float2 v = ml[g];
+      const float f = v.x == -__builtin_inff() ? 1.0f : exp2f(v.x - mm);
+      sum += v.y * f;
+      o += os[g][lane] * f;
+    }
+  }
   T* dst = static_cast<T*>(a.out.data) + b * a.out.seq_stride + (long long)(row / a.group) * a.out.token_stride +
-           (long long)(kvh * a.group + row % a.group) * a.out.head_stride + threadIdx.x;
-  if constexpr (std::is_same<T, float>::value)
-    *dst = y;
-  else
-    dst->bits = (uint16_t)bf16_of(y);
+           (long long)(kvh * a.group + row % a.group) * a.out.head_stride + 4 * lane;
+  store4(dst, o * (sum == 0.0f ? 0.0f : 1.0f / sum));
 }
 
-template <class T, int D, int CT>
-void run_attn(const Kv8AttnArgs& a, int batch, int groups, hipStream_t st) {
-  constexpr int kRows = CT * (std::is_same<T, float>::value ? 8 : 16);
-  hipLaunchKernelGGL((kv8_attn_kernel<T, D, CT>), dim3(a.nsplit * groups, a.c.kv_heads, batch), dim3(256), 0, st, a);
-  if (a.nsplit > 1)
-    hipLaunchKernelGGL((kv8_merge_kernel<T, D, kRows>), dim3(a.rows * a.group, a.c.kv_heads, batch), dim3(D), 0, st, a);
-}
 template <class T, int D>
 void run_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int batch, hipStream_t st) {
+  const dim3 grid(a.nsplit * p.groups, a.c.kv_heads, batch);
   if (p.tiles == 1)
-    run_attn<T, D, 1>(a, batch, p.groups, st);
+    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 1>), grid, dim3(256), 0, st, a);
   else if (p.tiles == 2)
-    run_attn<T, D, 2>(a, batch, p.groups, st);
+    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
   else
-    run_attn<T, D, 4>(a, batch, p.groups, st);
+    launch_kv8_attention_tiles(a, std::is_same<T, float>::value ? QWEN_TYPE_F32 : QWEN_TYPE_BF16, batch, p.groups, st);
+  const int R = a.rows * a.group, per_block = 1024 / D;
+  if (a.nsplit > 4)
+    hipLaunchKernelGGL((kv8_merge_kernel<T, D, true>), dim3(R, a.c.kv_heads, batch), dim3(256), 0, st, a);
+  else if (a.nsplit > 1)
+    hipLaunchKernelGGL((kv8_merge_kernel<T, D, false>), dim3((R + per_block - 1) / per_block, a.c.kv_heads, batch), dim3(256), 0, st, a);
 }
 
 template <class F>
@@ -602,15 +566,18 @@ void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, 
 }
 
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys) {
-  const int group = q_heads / c.kv_heads, per_tile = type == QWEN_TYPE_F32 ? 8 : 16;
-  const long long tiles = ((long long)rows * group + per_tile - 1) / per_tile;
+  const bool two = type == QWEN_TYPE_F32;
+  const long long R = (long long)rows * (q_heads / c.kv_heads);
+  const long long per_tile = two ? 8 : 16, tiles = (R + per_tile - 1) / per_tile;
   Kv8AttnPlan p{};
-  p.tiles = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-  p.groups = (int)((tiles + p.tiles - 1) / p.tiles);
+  p.tiles = tiles > 2 ? 4 : (int)tiles;
+  p.tile_rows = p.tiles == 4 ? kKv8TileRows : (int)(p.tiles * per_tile);
+  p.groups = (int)((R + p.tile_rows - 1) / p.tile_rows);
   const long long blocks = (max_keys + kKv8Block - 1) / kKv8Block;
   const long long others = (long long)p.groups * c.kv_heads * batch;
-  long long per = (blocks * others + 511) / 512;
-  if (per < 4) per = 4;
+  long long per = (blocks * others + 255) / 256;
+  if (p.tiles == 4 && others >= 160) per = blocks;
+  if (per < 4) per = blocks <= 12 ? blocks : 4;
   const long long least = (blocks + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (per < least) per = least;
   per = (per + 3) / 4 * 4;
@@ -635,6 +602,7 @@ void launch_kv8_attention(const qwen_kv8_cache& c, int type, const qwen_kv8_rows
   a.scale_log2e = scale * 1.44269504088896340736f;
   a.nsplit = p.nsplit;
   a.per_split = p.per_split;
+  a.tile_rows = p.tile_rows;
   a.part = static_cast<float*>(workspace);
   a.pml = reinterpret_cast<float2*>(a.part + (size_t)batch * q_heads * rows * p.nsplit * c.head_dim);
   by_type(type, c.head_dim, [&](auto t, auto d) { run_attn<decltype(t), decltype(d)::value>(a, p, batch, st); });
