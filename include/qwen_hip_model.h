@@ -31,6 +31,7 @@
 
 #include <stdint.h>
 
+#include "qwen_hip_kv8.h"
 #include "qwen_layout.h"
 
 #ifdef __cplusplus
@@ -135,6 +136,19 @@ int qwen_hip_model_prefill_layers(qwen_hip_model* m, int mode, int first_layer, 
                                   int seq_len, int past, float* hidden, float* k_cache, float* v_cache,
                                   uint64_t seq_stride, uint64_t layer_stride);
 
+/* FAST decode and (chunked) prefill of a layer range over an 8-bit K/V cache (qwen_hip_kv8.h) instead of the fp32
+ * one: the arguments are those of qwen_hip_model_decode_layers and qwen_hip_model_prefill_layers, `cache` is
+ * the cache of layer first_layer (2 KV heads of 128), and the caches of the following layers lie behind it,
+ * each array contiguous over the layers.  The new tokens' K/V rows are stored as codes first and the
+ * attention reads the codes, the new tokens' own included, so a prompt processed in chunks and in one
+ * piece see different roundings of its last blocks.  A sequence with a negative position in a decode is
+ * inactive: its cache is left as it is (its hidden row is overwritten).  `flags`: 0 or
+ * QWEN_FLAG_NO_BF16_ROUND.  qwen_hip_model_time_kernel does not follow these calls. */
+int qwen_hip_model_decode_kv8(qwen_hip_model* m, int flags, int first_layer, int layer_count, int batch, float* hidden,
+                              const int* positions, int max_keys, const qwen_kv8_cache* cache);
+int qwen_hip_model_prefill_kv8(qwen_hip_model* m, int flags, int first_layer, int layer_count, int batch, int seq_len,
+                               int past, float* hidden, const qwen_kv8_cache* cache);
+
 /* Embedding lookup from the model's bf16 table: hidden[i] = fp32(table[token_ids[i]]) (ids outside
  * [0, vocab) read row 0).  token_ids and hidden are device pointers. */
 int qwen_hip_model_embed(qwen_hip_model* m, const int* token_ids, int count, float* hidden);
@@ -158,6 +172,12 @@ int qwen_hip_model_logits(qwen_hip_model* m, const float* hidden, int count, flo
  * a NaN counts as the maximum), the logits being those of qwen_hip_model_logits (not stored).
  * Device pointers. */
 int qwen_hip_model_greedy(qwen_hip_model* m, const float* hidden, int count, int* token_ids);
+
+/* Next tokens drawn from the same logits (not stored), as qwen_hip_sample draws them (qwen_hip_sample.h):
+ * uniforms [count], and temperature, top_k, top_p, min_p [count] or null.  Device pointers. */
+int qwen_hip_model_sample(qwen_hip_model* m, const float* hidden, int count, const float* uniforms,
+                          const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                          int* token_ids);
 
 /* Re-runs one kernel of the most recent decode/prefill call `reps` times in isolation, on the
  * model's stream between two HIP events, with that call's shapes and the weights of `layer` (one of

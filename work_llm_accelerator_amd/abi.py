@@ -112,6 +112,9 @@ EXTRA_SIGNATURES: dict[str, tuple[list, object]] = {
     "qwen_hip_kv8_load": ([C8, c_int, R8, R8, c_int, c_int, c_int, P, P], c_int),
     "qwen_hip_kv8_attention_workspace": ([C8, c_int, c_int, c_int, c_int, c_int, U64P], c_int),
     "qwen_hip_kv8_attention": ([C8, c_int, R8, R8, c_int, c_int, c_int, P, c_int, ctypes.c_float, P, c_u64, P], c_int),
+    "qwen_hip_model_decode_kv8": ([P, c_int, c_int, c_int, c_int, P, P, c_int, C8], c_int),
+    "qwen_hip_model_prefill_kv8": ([P, c_int, c_int, c_int, c_int, c_int, c_int, P, C8], c_int),
+    "qwen_hip_model_sample": ([P, P, c_int, P, P, P, P, P, P], c_int),
     # token sampling (include/qwen_hip_sample.h)
     "qwen_hip_sample_workspace": ([c_int, c_int, U64P], c_int),
     "qwen_hip_sample": ([P, c_int, ctypes.c_int64, c_int, c_int, P, P, P, P, P, P, P, c_u64, P], c_int),

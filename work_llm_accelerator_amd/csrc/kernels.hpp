@@ -305,6 +305,12 @@ void launch_kv8_attention(const qwen_kv8_cache& c, int type, const qwen_kv8_rows
                           int batch, int rows, const int* positions, int max_keys, float scale, const Kv8AttnPlan& p,
                           void* workspace, hipStream_t st);
 
+// RoPE of the q and k heads of [q | k | v] rows in place: token t is token t % seq_len of sequence t / seq_len, at position
+// positions[t / seq_len] + t % seq_len (outside [0, limit): left as it is), rope [position][cos 64 | sin 64].
+void launch_rope_qk(float* qkv, int stride, int tokens, int seq_len, const int* positions, const float* rope, int limit,
+                    hipStream_t st);
+void launch_fill_i32(int* p, int n, int value, hipStream_t st);
+
 // ---- token sampling: kernels_sample.hip (arguments as in include/qwen_hip_sample.h, checked by the caller) ----
 struct SampleArgs {
   const void* logits;

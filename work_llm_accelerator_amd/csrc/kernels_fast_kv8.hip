@@ -151,6 +151,31 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(qwen_kv8_cache c, qwen_k
   }
 }
 
+// ---- the model's rows before they are stored ----
+// One block per token: 64 rotation pairs (p, p + 64) of each of the 14 q and k heads.
+__global__ void __launch_bounds__(256) rope_qk_kernel(float* __restrict__ qkv, int stride, int seq_len,
+                                                      const int* __restrict__ positions, const float* __restrict__ rope,
+                                                      int limit) {
+  const int t = blockIdx.x;
+  const long long pos = (long long)positions[t / seq_len] + t % seq_len;
+  if (pos < 0 || pos >= limit) return;
+  const int p = threadIdx.x & 63;
+  const float c = rope[(size_t)pos * 128 + p], s = rope[(size_t)pos * 128 + 64 + p];
+  float* row = qkv + (size_t)t * stride;
+#pragma unroll
+  for (int h = threadIdx.x >> 6; h < QWEN_Q_HEADS + QWEN_KV_HEADS; h += 4) {
+    float* x = row + h * QWEN_HEAD_DIM + p;
+    const float lo = x[0], hi = x[64];
+    x[0] = lo * c - hi * s;
+    x[64] = hi * c + lo * s;
+  }
+}
+
+__global__ void __launch_bounds__(256) fill_i32_kernel(int* __restrict__ p, int n, int value) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = value;
+}
+
 // ---- load -----------------------------------------------------------------------------------
 // The inverse, one block of 256 threads per (cache block, head, K or V, sequence); bound by the rows written.
 // grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
@@ -563,6 +588,15 @@ void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, 
     hipLaunchKernelGGL((kv8_load_kernel<decltype(t), decltype(d)::value>), dim3(touched, 2 * c.kv_heads, batch),
                        dim3(256), 0, st, c, k, v, rows, (int)zero_outside, positions);
   });
+}
+
+void launch_rope_qk(float* qkv, int stride, int tokens, int seq_len, const int* positions, const float* rope, int limit,
+                    hipStream_t st) {
+  hipLaunchKernelGGL(rope_qk_kernel, dim3(tokens), dim3(256), 0, st, qkv, stride, seq_len, positions, rope, limit);
+}
+
+void launch_fill_i32(int* p, int n, int value, hipStream_t st) {
+  hipLaunchKernelGGL(fill_i32_kernel, dim3((n + 255) / 256), dim3(256), 0, st, p, n, value);
 }
 
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys) {

@@ -11,6 +11,7 @@
 
 #include "kernels.hpp"
 #include "qwen_hip_model.h"
+#include "qwen_hip_sample.h"
 #include "runtime.hpp"
 
 using namespace qwen;
@@ -503,6 +504,77 @@ struct qwen_hip_model {
     QWEN_HIP(hipGetLastError());
   }
 
+  // FAST decode (S = 1 new token per sequence at positions `pos`) or prefill (S tokens at past..) over an 8-bit cache:
+  // `cache` is that of layer `first`, those of the following layers lie behind it.  The rows are projected,
+  // rotated, stored as codes, and the attention reads the codes, its own tokens' included.
+  void layers_kv8(int first, int count, int B, int S, bool prefill, int past, float* hidden, const int* pos, int max_keys,
+                  qwen_kv8_cache cache, int round) {
+    const int T = B * S;
+    const Kv8AttnPlan plan = plan_kv8_attention(cache, QWEN_TYPE_F32, QWEN_Q_HEADS, B, S, max_keys);
+    const size_t attn_bytes = (plan.workspace + 255u) & ~size_t(255u);
+    const Ws w = carve(T, 1, 1, attn_bytes + (size_t)B * 4u);
+    if (prefill) {
+      int* at = reinterpret_cast<int*>(w.kvt + attn_bytes);
+      launch_fill_i32(at, B, past, stream);
+      pos = at;
+    }
+    const float* rope = prefill ? rope_prefill : rope_decode;
+    const int norm = prefill ? kNormPrefill : kNormDecode;
+    const bool fused = T <= (prefill ? kPrefillFuseTokens : kSplitTokens);
+    const bool grouped = T <= kSkinnyTokens && (prefill || T > 1);
+    GemmArgs gq{}, fn{};
+    gq.xq_out = w.gxq;
+    gq.gsx_out = w.gsx;
+    gq.gcorr_out = w.gcorr;
+    fn.fuse = kFuseNormQuant;
+    fn.norm = norm;
+    fn.xq_out = w.xq;
+    fn.sx_out = w.sx;
+    fn.sums_out = w.sums;
+    const int64_t row = kQkvRows;
+    const qwen_kv8_rows q{w.qkv, S * row, row, QWEN_HEAD_DIM}, k{w.qkv + QWEN_HIDDEN, S * row, row, QWEN_HEAD_DIM},
+        v{w.qkv + QWEN_HIDDEN + QWEN_KV_WIDTH, S * row, row, QWEN_HEAD_DIM},
+        ctx{w.ctx, (int64_t)S * QWEN_HIDDEN, QWEN_HIDDEN, QWEN_HEAD_DIM};
+    const size_t blocks = (size_t)cache.sequences * cache.blocks * cache.kv_heads;
+    for (int i = 0; i < count; ++i) {
+      const FastLayer& f = fast[first + i];
+      if (!fused || i == 0)
+        launch_norm_quant(hidden, QWEN_HIDDEN, T, QWEN_HIDDEN, f.ln, norm, w.xq, w.sx, w.sums, nullptr, stream);
+      gemm(w, T, QWEN_HIDDEN, (int)kQkvRows, f.qkv, f.sw_qkv, f.b_qkv, w.qkv, kQkvRows, kEpiStore);
+      launch_rope_qk(w.qkv, (int)kQkvRows, T, S, pos, rope, max_keys, stream);
+      launch_kv8_store(cache, QWEN_TYPE_F32, k, v, B, S, pos, stream);
+      launch_kv8_attention(cache, QWEN_TYPE_F32, q, ctx, QWEN_Q_HEADS, B, S, pos, max_keys, 0.08838834764831845f, plan,
+                           w.kvt, stream);
+      launch_norm_quant(w.ctx, QWEN_HIDDEN, T, QWEN_HIDDEN, nullptr, kNormNone, w.xq, w.sx, w.sums, nullptr, stream);
+      fn.norm_w = f.post_ln;
+      gemm(w, T, QWEN_HIDDEN, QWEN_HIDDEN, f.o, f.sw_o, nullptr, w.att, QWEN_HIDDEN, kEpiStore, nullptr, nullptr,
+           nullptr, 0, 0, fused ? &fn : nullptr);
+      if (!fused)
+        launch_norm_quant(w.att, QWEN_HIDDEN, T, QWEN_HIDDEN, f.post_ln, norm, w.xq, w.sx, w.sums, nullptr, stream);
+      gemm(w, T, QWEN_HIDDEN, QWEN_INTERMEDIATE, f.gate, f.sw_gate, nullptr, w.s, QWEN_INTERMEDIATE, kEpiSiluMul, f.up,
+           f.sw_up, nullptr, 0, prefill ? 1 : 0, grouped ? &gq : nullptr);
+      if (!grouped)
+        launch_norm_quant(w.s, QWEN_INTERMEDIATE, T, QWEN_INTERMEDIATE, nullptr, kNormNone, w.xq, w.sx, w.sums, nullptr,
+                          stream);
+      const bool fuse_next = fused && i + 1 < count;  // the next layer's input RMSNorm + quantize
+      fn.norm_w = fuse_next ? fast[first + i + 1].ln : nullptr;
+      GemmArgs da = args(w, T, QWEN_INTERMEDIATE, QWEN_HIDDEN, f.down, f.sw_down, nullptr, hidden, QWEN_HIDDEN, nullptr,
+                         nullptr, w.att, round, 0, fuse_next ? &fn : nullptr);
+      if (grouped) {  // the down partials carry the per-group offsets: the reduce step gets zero sums
+        da.xq = w.gxq;
+        da.gsx = w.gsx;
+        da.gcorr = w.gcorr;
+        da.sums = w.zero_sums;
+      }
+      launch_gemm_i8(da, kEpiResidual, stream);
+      cache.k += blocks * QWEN_KV8_BLOCK * QWEN_HEAD_DIM;
+      cache.v += blocks * QWEN_KV8_BLOCK * QWEN_HEAD_DIM;
+      cache.k_scale += blocks;
+      cache.v_scale += blocks;
+    }
+    QWEN_HIP(hipGetLastError());
+  }
+
   void decode_ordered(int first, int count, int B, float* hidden, const int* pos, int max_keys, float* kc0,
                       float* vc0, uint64_t ss, uint64_t ls, int round) {
     float* att = scratch((size_t)B * QWEN_HIDDEN * 4u);
@@ -766,6 +838,51 @@ int qwen_hip_model_prefill(qwen_hip_model* m, int mode, int batch, int seq_len, 
   return qwen_hip_model_prefill_chunk(m, mode, batch, seq_len, 0, hidden, k_cache, v_cache, seq_stride, layer_stride);
 }
 
+// `c` as the cache of a layer range of this model, holding `keys` tokens of `batch` sequences.
+static const char* kv8_model_problem(const qwen_kv8_cache* c, int batch, int64_t keys) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return "null cache";
+  if (c->kv_heads != QWEN_KV_HEADS || c->head_dim != QWEN_HEAD_DIM) return "the model's 8-bit cache has 2 KV heads of 128";
+  if (c->sequences < batch || c->blocks < 1 || c->blocks > (1 << 24) || keys > (int64_t)c->blocks * QWEN_KV8_BLOCK)
+    return "8-bit cache too small for max_keys / batch";
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) return "the codes of an 8-bit cache must be 16-byte aligned";
+  if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3u) return "the scales of an 8-bit cache must be 4-byte aligned";
+  return nullptr;
+}
+
+int qwen_hip_model_decode_kv8(qwen_hip_model* m, int flags, int first_layer, int layer_count, int batch, float* hidden,
+                              const int* positions, int max_keys, const qwen_kv8_cache* cache) {
+  if (!m || !hidden || !positions) return invalid("null argument");
+  if (first_layer < 0 || layer_count <= 0 || first_layer > m->layers - layer_count) return invalid("invalid layer range");
+  if (flags & ~QWEN_FLAG_NO_BF16_ROUND) return invalid("unknown flags (the 8-bit cache has the FAST mode only)");
+  if (batch <= 0 || (size_t)batch > kMaxDecodeBatch || max_keys <= 0 || max_keys > QWEN_MAX_SEQ) return invalid("invalid decode shape");
+  if (const char* why = kv8_model_problem(cache, batch, max_keys)) return invalid(why);
+  std::lock_guard<std::mutex> lock(m->mu);
+  return guarded_model([&]() -> int {
+    m->layers_kv8(first_layer, layer_count, batch, 1, false, 0, hidden, positions, max_keys, *cache,
+                  (flags & QWEN_FLAG_NO_BF16_ROUND) ? 0 : 1);
+    m->last = LastCall{};
+    return QWEN_OK;
+  });
+}
+
+int qwen_hip_model_prefill_kv8(qwen_hip_model* m, int flags, int first_layer, int layer_count, int batch, int seq_len,
+                               int past, float* hidden, const qwen_kv8_cache* cache) {
+  if (!m || !hidden) return invalid("null argument");
+  if (first_layer < 0 || layer_count <= 0 || first_layer > m->layers - layer_count) return invalid("invalid layer range");
+  if (flags & ~QWEN_FLAG_NO_BF16_ROUND) return invalid("unknown flags (the 8-bit cache has the FAST mode only)");
+  if (batch <= 0 || (size_t)batch > kMaxDecodeBatch || seq_len <= 0 || seq_len > QWEN_MAX_SEQ || past < 0 ||
+      past > QWEN_MAX_SEQ - seq_len || (int64_t)batch * seq_len > (1 << 24))
+    return invalid("invalid prefill shape (at most 2^24 tokens) or past length");
+  if (const char* why = kv8_model_problem(cache, batch, (int64_t)past + seq_len)) return invalid(why);
+  std::lock_guard<std::mutex> lock(m->mu);
+  return guarded_model([&]() -> int {
+    m->layers_kv8(first_layer, layer_count, batch, seq_len, true, past, hidden, nullptr, past + seq_len, *cache,
+                  (flags & QWEN_FLAG_NO_BF16_ROUND) ? 0 : 1);
+    m->last = LastCall{};
+    return QWEN_OK;
+  });
+}
+
 int qwen_hip_model_embed(qwen_hip_model* m, const int* token_ids, int count, float* hidden) {
   if (!m || !token_ids || !hidden || count <= 0) return invalid("invalid embed arguments");
   if (!m->embed) return invalid("model has no embedding table (synthetic models, or qwen_hip_model_set_head)");
@@ -820,6 +937,34 @@ int qwen_hip_model_logits(qwen_hip_model* m, const float* hidden, int count, flo
 int qwen_hip_model_greedy(qwen_hip_model* m, const float* hidden, int count, int* token_ids) {
   if (!token_ids) return invalid("invalid token id buffer");
   return run_head(m, hidden, count, nullptr, token_ids);
+}
+
+int qwen_hip_model_sample(qwen_hip_model* m, const float* hidden, int count, const float* uniforms,
+                          const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                          int* token_ids) {
+  if (!m || !hidden || count <= 0 || count > (1 << 20)) return invalid("invalid head arguments");
+  if (!uniforms || !token_ids) return invalid("null sampling argument");
+  if (!m->embed || !m->head_norm) return invalid("model has no head (synthetic models, or qwen_hip_model_set_head)");
+  std::lock_guard<std::mutex> lock(m->mu);
+  return guarded_model([&]() -> int {
+    // the logits of at most kSampleRows tokens at a time (256 rows of 151936: 156 MB)
+    constexpr int kSampleRows = 256;
+    auto align = [](size_t n) { return (n + 255u) & ~size_t(255u); };
+    const int rows = count < kSampleRows ? count : kSampleRows;
+    const size_t head = align(head_workspace_bytes(rows, m->vocab)), logit_bytes = align((size_t)rows * m->vocab * 4u);
+    char* ws = static_cast<char*>(m->head_ws.get(head + logit_bytes + sample_workspace_bytes(rows, m->vocab)));
+    float* logits = reinterpret_cast<float*>(ws + head);
+    for (int i = 0; i < count; i += rows) {
+      const int n = count - i < rows ? count - i : rows;
+      launch_head(hidden + (size_t)i * QWEN_HIDDEN, n, m->head_norm, m->embed, m->vocab, ws, logits, nullptr, m->stream);
+      launch_sample(SampleArgs{logits, QWEN_TYPE_F32, m->vocab, n, m->vocab, uniforms + i, temperature ? temperature + i : nullptr,
+                               top_k ? top_k + i : nullptr, top_p ? top_p + i : nullptr, min_p ? min_p + i : nullptr,
+                               token_ids + i},
+                    ws + head + logit_bytes, m->stream);
+    }
+    QWEN_HIP(hipGetLastError());
+    return QWEN_OK;
+  });
 }
 
 int qwen_hip_model_time_kernel(qwen_hip_model* m, int kernel, int layer, int reps, float* avg_ms) {

@@ -156,6 +156,39 @@ class DeviceModel:
                                                     cache.layer_stride)
         _check(self.lib, st, "qwen_hip_model_prefill_layers")
 
+    def _range_kv8(self, cache, layers):
+        """(first layer, layer count, struct of that layer's cache) of a `layers` range over a Kv8Cache."""
+        if layers is None:
+            first, count = 0, self.layers
+        elif isinstance(layers, int):
+            first, count = layers, 1
+        else:
+            first, count = int(layers[0]), int(layers[1])
+        if cache.layers != self.layers and cache.layers < count:
+            raise ValueError(f"cache holds {cache.layers} layers, the range {count}")
+        return first, count, cache.layer_struct(first if cache.layers == self.layers else 0)
+
+    def decode_kv8(self, hidden, positions, max_keys: int, cache, flags: int = 0, order: bool = True,
+                   layers=None) -> None:
+        """FAST decode over an 8-bit cache (kv8.Kv8Cache): hidden [B,1536] fp32 (in/out), positions [B] int32 on the
+        GPU (negative: inactive); flags 0 or FLAG_NO_BF16_ROUND; `layers` as in _range."""
+        if order:
+            self._enter()
+        first, count, c = self._range_kv8(cache, layers)
+        st = self.lib.qwen_hip_model_decode_kv8(self.handle, flags, first, count, hidden.shape[0], _ptr(hidden),
+                                                _ptr(positions), int(max_keys), ctypes.byref(c))
+        _check(self.lib, st, "qwen_hip_model_decode_kv8")
+
+    def prefill_kv8(self, hidden, cache, flags: int = 0, order: bool = True, past: int = 0, layers=None) -> None:
+        """FAST prefill over an 8-bit cache: hidden [B,S,1536] fp32 (in/out) at positions past..past+S-1, whose K/V
+        are stored as codes (tokens 0..past-1 are there already); flags and `layers` as in decode_kv8."""
+        if order:
+            self._enter()
+        first, count, c = self._range_kv8(cache, layers)
+        st = self.lib.qwen_hip_model_prefill_kv8(self.handle, flags, first, count, hidden.shape[0], hidden.shape[1],
+                                                 int(past), _ptr(hidden), ctypes.byref(c))
+        _check(self.lib, st, "qwen_hip_model_prefill_kv8")
+
     def embed(self, token_ids, hidden, order: bool = True) -> None:
         if order:
             self._enter()
@@ -194,6 +227,19 @@ class DeviceModel:
         n = hidden.numel() // 1536
         st = self.lib.qwen_hip_model_greedy(self.handle, _ptr(hidden), n, _ptr(token_ids))
         _check(self.lib, st, "qwen_hip_model_greedy")
+
+    def sample(self, hidden, uniforms, token_ids, temperature=None, top_k=None, top_p=None, min_p=None,
+               order: bool = True) -> None:
+        """Next token ids [N] int32 of hidden [N,1536], drawn from the logits by uniforms [N] in [0, 1) with
+        temperature, top-k, top-p and min-p [N] (None: off), as sampling.sample_logits draws them."""
+        from .sampling import row_params
+
+        n = hidden.numel() // 1536
+        params = row_params(n, hidden.device, uniforms, temperature, top_k, top_p, min_p, token_ids)
+        if order:
+            self._enter()
+        st = self.lib.qwen_hip_model_sample(self.handle, _ptr(hidden), n, *params)
+        _check(self.lib, st, "qwen_hip_model_sample")
 
     def time_kernel(self, kernel: int, layer: int = 0, reps: int = 20) -> float:
         """Mean milliseconds of one launch of `kernel`, re-run in isolation with the shapes of the
