@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(256) fill_i32_kernel(int* __restrict__ p, int 
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv8_rows kout, qwen_kv8_rows vout, int rows,
                                                        int zero_outside, const int* __restrict__ positions) {
-  constexpr int kPer = D / 8, kStep = 256 / kPer, kPasses = kKv8Block / kStep;
+  constexpr int kVec = 16 / sizeof(T);  // elements of a 16-byte store: a wave writes whole rows at a time
+  constexpr int kPer = D / kVec, kStep = 256 / kPer, kPasses = kKv8Block / kStep;
   __shared__ uint32_t tile[kKv8Block][D / 4 + 2];
   const int b = blockIdx.z, h = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv
   const int t0 = first < 0 ? (int)-first : 0, t1 = last > rows ? (int)(rows - first) : kKv8Block;
   const qwen_kv8_rows out = is_v ? vout : kout;
   T* dst = static_cast<T*>(out.data) + b * out.seq_stride + h * out.head_stride;
-  const int tid = threadIdx.x, d8 = (tid % kPer) * 8;
+  const int tid = threadIdx.x, d0 = (tid % kPer) * kVec;
   const size_t place = inside ? ((size_t)b * c.blocks + (size_t)blk) * c.kv_heads + h : 0;
   const int8_t* src = (is_v ? c.v : c.k) + place * (size_t)(kKv8Block * D);
   const float s = inside ? (is_v ? c.v_scale : c.k_scale)[place] : 0.0f;
@@ -222,17 +223,21 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv
   for (int p = 0; p < kPasses; ++p) {
     const int t = p * kStep + tid / kPer;
     if (t < t0 || t >= t1) continue;
-    uint2 w = make_uint2(0u, 0u);
+    uint32_t w[kVec / 4] = {};
     if (inside) {
-      if (is_v)
-        w = make_uint2(tile[t][d8 / 4], tile[t][d8 / 4 + 1]);
-      else
-        w = *reinterpret_cast<const uint2*>(src + ((d8 >> 6) * kKv8Block + t) * 64 + (d8 & 63));
-    }
-    float x[8];
+      const int8_t* at = src + ((d0 >> 6) * kKv8Block + t) * 64 + (d0 & 63);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)code_byte(i < 4 ? w.x : w.y, i & 3) * s;
-    store8(dst + (first + t) * out.token_stride + d8, x);
+      for (int i = 0; i < kVec / 4; ++i) w[i] = is_v ? tile[t][d0 / 4 + i] : reinterpret_cast<const uint32_t*>(at)[i];
+    }
+    T* to = dst + (first + t) * out.token_stride + d0;
+    if constexpr (kVec == 8) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)code_byte(w[i >> 2], i & 3) * s;
+      store8(to, x);
+    } else {
+      store4(to, f32x4{(float)code_byte(w[0], 0), (float)code_byte(w[0], 1), (float)code_byte(w[0], 2), (float)code_byte(w[0], 3)} * s);
+    }
   }
 }
 
@@ -242,7 +247,13 @@ __device__ __forceinline__ float other_half(float x) {
   return bits_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_bits(x), 0x128, 0xF, 0xF, false));
 }
 
-constexpr float kProbBits = 15.0f;  // probabilities times 2^15: fp16 holds them normal down to 2^-29 of the largest
+// Maximum over the four lanes of a column (16 apart).
+__device__ __forceinline__ float column_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_bits(x), f32_bits(x), false, false);
+  x = fmaxf(bits_f32(a[0]), bits_f32(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(x), false, false);
+  return fmaxf(bits_f32(b[0]), bits_f32(b[1]));
+}
 
 // 16 bytes of the cache that nothing else reads (64 x 4096 fp32: 26.0 us, with cached loads 25.3 to 28.7).
 __device__ __forceinline__ uint4 load_once(const int8_t* p) {
@@ -262,7 +273,7 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
 // columns then carry the hi and lo terms of the probabilities.
 // grid = (nsplit * tile groups, kv_heads, batch), block = 256.
 template <class T, int D, int CT>
-__global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) kv8_attn_kernel(Kv8AttnArgs a) {
   constexpr bool kTwo = std::is_same<T, float>::value;
   constexpr int kRowsPerTile = kTwo ? 8 : 16, kHalves = D / 64, kDimTiles = D / 16;
   __shared__ float2 ml[4][CT * 16];
@@ -304,10 +315,10 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
     }
     top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    // times a power of two that brings the row's largest magnitude to [2^13, 2^14)
+    // times a power of two that brings the row's largest magnitude to [2^13, 2^14), and the scale's sign
     const int ex = min(253, max(13, 267 - (int)(top >> 23)));
-    const float up = bits_f32((uint32_t)ex << 23);
-    factor[ct] = top >= 0x7F800000u ? f32_nan() : a.scale_log2e * bits_f32((uint32_t)(254 - ex) << 23);
+    const float up = bits_f32(((uint32_t)ex << 23) | (f32_bits(a.scale_log2e) & 0x80000000u));
+    factor[ct] = top >= 0x7F800000u ? f32_nan() : fabsf(a.scale_log2e) * bits_f32((uint32_t)(254 - ex) << 23);
 #pragma unroll
     for (int s = 0; s < 2 * kHalves; ++s)
 #pragma unroll
@@ -322,6 +333,7 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
     for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  const float low_term = kTwo && col >= 8 ? 1.0f : 0.0f;
   const size_t block_bytes = (size_t)kKv8Block * D, head0 = (size_t)b * a.c.blocks * a.c.kv_heads + kvh;
   uint4 kr[4][kHalves], vr[kDimTiles];
   auto load_k = [&](int blk) {
@@ -368,26 +380,31 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
     float sv_col[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const float f = factor[ct] * sk;
-      float top = -__builtin_inff();
+      if constexpr (kTwo)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x = s[ct][t][i];
-          if constexpr (kTwo) x += other_half(x);
-          x *= f;
-          if (edge && blk * kKv8Block + 16 * t + 4 * g + i >= keys[ct]) x = -__builtin_inff();
-          s[ct][t][i] = x;
-          top = fmaxf(top, x);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      // a column that attends none of the block's tokens takes nothing from it, whatever its scale holds
-      sv_col[ct] = top == -__builtin_inff() ? 0.0f : sv;
-      const float mn = fmaxf(m[ct], top);
-      if (__any(mn > m[ct])) {
-        const float alpha = mn > m[ct] ? exp2f(m[ct] - mn) : 1.0f;
+          for (int i = 0; i < 4; ++i) s[ct][t][i] += other_half(s[ct][t][i]);
+      if (edge)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (blk * kKv8Block + 16 * t + 4 * g + i >= keys[ct]) s[ct][t][i] = -__builtin_inff();
+      float top = s[ct][0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[ct][e >> 2][e & 3]);
+      top = column_max(top);
+      // a column that attends none of the block's tokens takes nothing from it, whatever its scales hold
+      const bool none = top == -__builtin_inff();
+      float f = factor[ct] * sk;
+      f = none || f < 1.0e-37f ? 1.0e-37f : f;  // (a scale of 0 times a masked -inf would be NaN)
+      sv_col[ct] = none ? 0.0f : sv;
+      top *= f;
+      // the accumulators follow the maximum only once it is more than 2^4 ahead
+      if (!__all(top <= m[ct] + kProbLag && m[ct] > -__builtin_inff())) {
+        const bool up = top > m[ct] + kProbLag || (m[ct] == -__builtin_inff() && top > m[ct]);
+        const float mn = up ? top : m[ct], alpha = up ? __builtin_amdgcn_exp2f(m[ct] - mn) : 1.0f;
         l[ct] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < kDimTiles; ++dt) o[ct][dt] *= alpha;
@@ -395,14 +412,20 @@ __global__ void __launch_bounds__(256) kv8_attn_kernel(Kv8AttnArgs a) {
       }
       const float base = m[ct] == -__builtin_inff() ? 0.0f : m[ct] - kProbBits;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = __builtin_amdgcn_exp2f(s[ct][t][i] - base);
-          l[ct] += x;
-          const _Float16 hi = (_Float16)x;
-          p[ct][t >> 1][4 * (t & 1) + i] = kTwo && col >= 8 ? (_Float16)(x - (float)hi) : hi;
+      for (int e = 0; e < 16; e += 2) {
+        f32x2 x = {__builtin_amdgcn_exp2f(fmaf(s[ct][e >> 2][e & 3], f, -base)),
+                   __builtin_amdgcn_exp2f(fmaf(s[ct][e >> 2][(e & 3) + 1], f, -base))};
+        l[ct] += x[0];
+        l[ct] += x[1];
+        if constexpr (kTwo) {  // columns from 8 on: what the others' rounding leaves
+          const half2v hi = __builtin_convertvector(x, half2v);
+          x[0] = fmaf(-(float)hi[0], low_term, x[0]);
+          x[1] = fmaf(-(float)hi[1], low_term, x[1]);
         }
+        const half2v y = __builtin_convertvector(x, half2v);
+        p[ct][e >> 3][e & 7] = y[0];
+        p[ct][e >> 3][(e & 7) + 1] = y[1];
+      }
     }
 #pragma unroll
     for (int dt = 0; dt < kDimTiles; ++dt) {

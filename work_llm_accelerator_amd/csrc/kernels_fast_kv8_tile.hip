@@ -14,13 +14,9 @@
 namespace qwen {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
-// Probabilities enter the product times 2^11 relative to a maximum that may lag the true one by a factor of 2^4
-// (so that O is rescaled rarely): up to 2^15, and normal in fp16 down to 2^-25 of the largest.
-constexpr float kTileProbBits = 11.0f, kTileLag = 4.0f;
 constexpr int kTileFold = 6;  // V scales down to 2^-6 of the accumulator's unit go into the probabilities
 
 __device__ __forceinline__ float swap_max(float x) {  // maximum over the two lanes of a column
@@ -269,19 +265,19 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
     sum = 0.0f;
     // the block's V scale is folded into the probabilities where it is a little below the accumulator's unit
     shift = unit - sv;
-    base = m - kTileProbBits + (float)shift;
-    const bool usual = most <= m + kTileLag && m > -__builtin_inff() && (uint32_t)shift <= (uint32_t)kTileFold;
+    base = m - kProbBits + (float)shift;
+    const bool usual = most <= m + kProbLag && m > -__builtin_inff() && (uint32_t)shift <= (uint32_t)kTileFold;
     if (__all(usual)) return;
-    const bool first = m == -__builtin_inff(), up = most > m + kTileLag || (first && most > m);
+    const bool first = m == -__builtin_inff(), up = most > m + kProbLag || (first && most > m);
     const float mn = up ? most : m;
     const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
     // else the unit changes to it, unless none of its probabilities is large enough to be more than 0
-    const bool touched = most > mn - (kTileProbBits + 25.0f);
+    const bool touched = most > mn - (kProbBits + 25.0f);
     const bool change = touched && (first || ((uint32_t)shift > (uint32_t)kTileFold && shift <= 80));
     const float grow = __builtin_amdgcn_ldexpf(alpha, change && !first ? shift : 0);
     unit = change ? sv : unit;
     shift = change ? 0 : shift < 0 ? 400 : shift;
-    base = mn == -__builtin_inff() ? 0.0f : mn - kTileProbBits + (float)shift;
+    base = mn == -__builtin_inff() ? 0.0f : mn - kProbBits + (float)shift;
     m = mn;
     l *= alpha;
 #pragma unroll

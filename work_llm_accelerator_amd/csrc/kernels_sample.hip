@@ -7,7 +7,8 @@
 // Six launches, each over all rows: the row's maximum and minimum; a histogram (counts and weights) over 2048 equal
 // steps of the logit below the maximum; a list of the tokens of the steps in which top-k and top-p cut; the exact
 // (T, n) from that list; the kept weight of each segment of the row; the draw.  Rows are split over many blocks
-// except in the two launches that end in one number (the cut and the draw).
+// except in the two launches that end in one number (the cut and the draw).  A row with a small k lists everything
+// down to the step of its cut: its weights are those of the list only, and the draw is made from it too.
 #include <hip/hip_runtime.h>
 
 #include "kernels.hpp"
@@ -20,8 +21,10 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kBuckets = 2048;
 constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row)
+constexpr int kSmall = 2048;    // largest k whose row is decided by its list
 constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kThreads * 512 tokens)
 constexpr int kMaxChunks = 256;
+constexpr int kRed = kThreads / 64;  // words for the waves of a block (and two a wave of the chunks' maxima)
 constexpr uint32_t kUnlisted = 0xFFFFFFFFu;
 constexpr int kChunkThreads = 256;
 constexpr int kHistThreads = 512;
@@ -39,16 +42,49 @@ struct Cut {       // a kept set: key > key, and the first `ties` tokens with ke
   uint32_t ties;
 };
 
+// The value of the lane that DPP control kCtrl names, 0 where there is none or its row is not in kRows.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, kCtrl, kRows, 0xF, false);
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ u64 dpp(u64 x) {
+  return ((u64)dpp<kCtrl, kRows>((uint32_t)(x >> 32)) << 32) | dpp<kCtrl, kRows>((uint32_t)x);
+}
+// Running sum (or maximum) over the wave's lanes, this one included: shifts by 1, 2, 4, 8 within rows of 16, then each
+// row's last lane to the rows after it.  (A shuffle through LDS takes several times as long, and these launches
+// are chains of such steps.)
+template <class V, class F>
+__device__ __forceinline__ V wave_running(V x, F&& f) {
+  x = f(x, dpp<0x111, 0xF>(x));
+  x = f(x, dpp<0x112, 0xF>(x));
+  x = f(x, dpp<0x114, 0xF>(x));
+  x = f(x, dpp<0x118, 0xF>(x));
+  x = f(x, dpp<0x142, 0xA>(x));
+  return f(x, dpp<0x143, 0xC>(x));
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V x) {
+  return wave_running(x, [](V a, V b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ u64 last_lane(u64 x) { return ((u64)last_lane((uint32_t)(x >> 32)) << 32) | last_lane((uint32_t)x); }
+template <class V>
+__device__ __forceinline__ V wave_sum(V x) {
+  return last_lane(wave_scan(x));
+}
+__device__ __forceinline__ u64 wave_max(u64 x) {
+  return last_lane(wave_running(x, [](u64 a, u64 b) { return a > b ? a : b; }));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  return last_lane(wave_running(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; }));
+}
+
 // Sum over the block's threads (N) and the sum of the threads before (exclusive).
 template <int N>
 __device__ u64 block_scan(u64 x, u64* red, u64& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 inc = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const u64 o = __shfl_up(inc, off, 64);
-    if (lane >= off) inc += o;
-  }
+  const u64 inc = wave_scan(x);
   __syncthreads();
   if (lane == 63) red[wave] = inc;
   __syncthreads();
@@ -68,12 +104,13 @@ struct RowSpace {
   u64 weights[kBuckets];      // histogram
   uint32_t counts[kBuckets];
   u64 best[kMaxChunks];       // (key << 32 | ~index) of each chunk's maximum
-  float low[kMaxChunks];      // least finite logit
-  uint32_t list[kList];       // keys of the tokens of the steps with a cut
+  uint32_t low[kMaxChunks];   // ~key of the least finite logit
+  u64 list[kList];            // (key << 32 | index) of the tokens of the steps with a cut
   uint32_t listed;
   int k_step, p_low, p_high;  // the steps in the list (Needed)
   u64 k_before;
   Cut cut;
+  int drawn;                  // the row's token is written
 };
 
 struct Sampler {
@@ -130,26 +167,27 @@ struct Row {
   int unit_bits;
   bool greedy;
 
-  // Whole blocks of at least 256 threads (a multiple of 64); red: one u64 and one float per wave.
-  __device__ Row(const Sampler& s, int row, u64* red, float* redf) {
+  // Whole blocks of at least 256 threads (a multiple of 64); red: two words per wave.
+  __device__ Row(const Sampler& s, int row, u64* red) {
     u64 best = 0;
-    float low = __builtin_inff();
+    uint32_t low_key = 0;  // (~key: the largest is the least logit; 0: no finite logit)
     const RowSpace& w = s.space[row];
-    if ((int)threadIdx.x < s.chunks) best = w.best[threadIdx.x], low = w.low[threadIdx.x];
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const u64 o = __shfl_xor(best, off, 64);
-      best = o > best ? o : best;
-      low = fminf(low, __shfl_xor(low, off, 64));
-    }
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best, redf[threadIdx.x >> 6] = low;
+    temperature = s.a.temperature ? s.a.temperature[row] : 1.0f;
+    if ((int)threadIdx.x < s.chunks) best = w.best[threadIdx.x], low_key = w.low[threadIdx.x];
+    best = wave_max(best);
+    low_key = wave_max(low_key);
+    if ((threadIdx.x & 63) == 0 && threadIdx.x < kMaxChunks) red[threadIdx.x >> 6] = best, red[kMaxChunks / 64 + (threadIdx.x >> 6)] = low_key;
     __syncthreads();
-    for (int i = 0; i < kMaxChunks / 64; ++i) best = red[i] > best ? red[i] : best, low = fminf(low, redf[i]);
+#pragma unroll
+    for (int i = 0; i < kMaxChunks / 64; ++i) {
+      best = red[i] > best ? red[i] : best;
+      low_key = max(low_key, (uint32_t)red[kMaxChunks / 64 + i]);
+    }
     __syncthreads();
     top_key = (uint32_t)(best >> 32);
     top_index = (int)~(uint32_t)best;
+    const float low = low_key ? logit_of_key(~low_key) : __builtin_inff();
     top = logit_of_key(top_key);
-    temperature = s.a.temperature ? s.a.temperature[row] : 1.0f;
     greedy = !(temperature > 0.0f) || top_key == 0xFFFFFFFFu || !(fabsf(top) <= 3.402823466e38f);
     dtop = top, per_unit = 1.44269504088896340735992468100 / (double)temperature, unit_bits = s.unit_bits;
     const float range = fminf(s.spread * temperature, top - low);
@@ -185,30 +223,26 @@ __device__ __forceinline__ void over_chunk(const T* x, int vocab, int per, F&& f
 // grid = (chunks, rows).  Also clears the row's histogram.
 template <class T>
 __global__ void __launch_bounds__(kChunkThreads) sample_max_kernel(Sampler s) {
-  __shared__ u64 red[kChunkThreads / 64];
-  __shared__ float redf[kChunkThreads / 64];
+  __shared__ u64 red[kRed];
   const int row = blockIdx.y, tid = threadIdx.x;
   const T* x = row_of<T>(s.a, row);
   RowSpace& w = s.space[row];
   for (int i = blockIdx.x * kChunkThreads + tid; i < kBuckets; i += gridDim.x * kChunkThreads) w.weights[i] = 0, w.counts[i] = 0;
   if (blockIdx.x == 0 && tid == 0) w.listed = 0;
   u64 best = 0;
-  float low = __builtin_inff();
+  uint32_t low = 0;
   over_chunk<kChunkThreads>(x, s.a.vocab, s.per_chunk, [&](float v, int i) {
-    const u64 k = ((u64)order_key(v) << 32) | (u64)(~(uint32_t)i);
+    const uint32_t key = order_key(v);
+    const u64 k = ((u64)key << 32) | (u64)(~(uint32_t)i);
     best = k > best ? k : best;
-    if (v > -__builtin_inff()) low = fminf(low, v);
+    if (v > -__builtin_inff()) low = max(low, ~key);
   });
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const u64 o = __shfl_xor(best, off, 64);
-    best = o > best ? o : best;
-    low = fminf(low, __shfl_xor(low, off, 64));
-  }
-  if ((tid & 63) == 0) red[tid >> 6] = best, redf[tid >> 6] = low;
+  best = wave_max(best);
+  low = wave_max(low);
+  if ((tid & 63) == 0) red[tid >> 6] = best, red[kMaxChunks / 64 + (tid >> 6)] = low;
   __syncthreads();
   if (tid != 0) return;
-  for (int i = 1; i < kChunkThreads / 64; ++i) best = red[i] > best ? red[i] : best, low = fminf(low, redf[i]);
+  for (int i = 1; i < kChunkThreads / 64; ++i) best = red[i] > best ? red[i] : best, low = max(low, (uint32_t)red[kMaxChunks / 64 + i]);
   w.best[blockIdx.x] = best;
   w.low[blockIdx.x] = low;
 }
@@ -217,6 +251,7 @@ __device__ __forceinline__ bool wants_top_k(const Sampler& s, int row, int& k) {
   k = s.a.top_k ? s.a.top_k[row] : 0;
   return k > 0 && k < s.a.vocab;
 }
+__device__ __forceinline__ bool small_k(bool top_k, int k) { return top_k && k <= kSmall; }
 __device__ __forceinline__ bool wants_top_p(const Sampler& s, int row, float& p) {
   p = s.a.top_p ? s.a.top_p[row] : 1.0f;
   return p < 1.0f;
@@ -227,14 +262,14 @@ template <class T>
 __global__ void __launch_bounds__(kHistThreads) sample_hist_kernel(Sampler s) {
   __shared__ u64 weights[kBuckets];
   __shared__ uint32_t counts[kBuckets];
-  __shared__ u64 red[kHistThreads / 64];
-  __shared__ float redf[kHistThreads / 64];
+  __shared__ u64 red[kRed];
   const int row = blockIdx.y, tid = threadIdx.x;
   int k;
   float p;
-  const bool top_p = wants_top_p(s, row, p);
-  if (!wants_top_k(s, row, k) && !top_p) return;
-  const Row r(s, row, red, redf);
+  const bool top_p = wants_top_p(s, row, p), top_k = wants_top_k(s, row, k);
+  if (!top_k && !top_p) return;
+  const bool weigh = top_p && !small_k(top_k, k);
+  const Row r(s, row, red);
   if (r.greedy) return;
   for (int i = tid; i < kBuckets; i += kHistThreads) weights[i] = 0, counts[i] = 0;
   __syncthreads();
@@ -242,7 +277,7 @@ __global__ void __launch_bounds__(kHistThreads) sample_hist_kernel(Sampler s) {
   over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int) {
     const int b = r.step(v);
     atomicAdd(&counts[b], 1u);
-    if (top_p) {
+    if (weigh) {
       const u64 n = r.fixed(v);
       if (n) atomicAdd(&weights[b], n);
     }
@@ -333,6 +368,11 @@ __device__ Needed needed_steps(const Held<N>& h, bool top_k, int k, bool top_p, 
   if (top_k) {
     const auto f = h.find(false, (u64)k, 0.0, kBuckets, 0, pick, pick_step);
     if (f.step < kBuckets - 1) n.k_step = f.step, n.k_before = f.before, at = f.at, tokens = f.tokens;
+    if (small_k(top_k, k)) {  // everything with weight down to the cut
+      n.low = 0, n.high = min(f.step, kBuckets - 2);
+      n.listed = f.before + tokens <= (u64)kList;
+      return n;
+    }
   }
   if (top_p) {
     const int last = n.k_step < 0 ? kBuckets : n.k_step;
@@ -349,13 +389,12 @@ __device__ Needed needed_steps(const Held<N>& h, bool top_k, int k, bool top_p, 
   return n;
 }
 
-// Lists the keys of the needed steps' tokens; every block finds the steps for itself.  grid = (chunks, rows).
+// Lists the needed steps' tokens; every block finds the steps for itself.  grid = (chunks, rows).
 template <class T>
 __global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
-  __shared__ u64 red[kHistThreads / 64], pick[4];
-  __shared__ float redf[kHistThreads / 64];
+  __shared__ u64 red[kRed], pick[4];
   __shared__ uint32_t pick_step, found, at;
-  __shared__ uint32_t keys[kList];
+  __shared__ u64 keys[kList];
   const int row = blockIdx.y, tid = threadIdx.x;
   int k;
   float p;
@@ -363,7 +402,7 @@ __global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
   if (!top_k && !top_p) return;
   RowSpace& w = s.space[row];
   Held<kHistThreads> held(w);
-  const Row r(s, row, red, redf);
+  const Row r(s, row, red);
   if (r.greedy) return;
   held.scan(red);
   if (tid == 0) found = 0u;
@@ -374,161 +413,13 @@ __global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
   }
   if (!need.listed) return;
   const T* x = row_of<T>(s.a, row);
-  over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int) {
-    if (need.has(r.step(v))) keys[atomicAdd(&found, 1u)] = order_key(v);
+  over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int i) {
+    if (need.has(r.step(v))) keys[atomicAdd(&found, 1u)] = ((u64)order_key(v) << 32) | (u64)(uint32_t)i;
   });
   __syncthreads();
   if (tid == 0 && found) at = atomicAdd(&w.listed, found);  // one a block: they are serialized over the row
   __syncthreads();
   for (int i = tid; i < (int)found; i += kHistThreads) w.list[at + i] = keys[i];
-}
-
-// The cuts of one row: grid = rows.
-template <class T>
-__global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
-  __shared__ u64 hist[kBuckets];
-  __shared__ uint32_t count[kBuckets];
-  __shared__ uint32_t list[kList];
-  __shared__ u64 red[kChunkThreads / 64], pick[4];
-  __shared__ float redf[kChunkThreads / 64];
-  __shared__ uint32_t pick_step, differ, sample_key;
-  const int row = blockIdx.x, tid = threadIdx.x, vocab = s.a.vocab;
-  Cut cut{0u, 0u};  // everything: every key is above 0 (-inf has key 0x007FFFFF)
-  int k;
-  float p;
-  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
-  RowSpace& w = s.space[row];
-  if (!top_k && !top_p) {
-    if (tid == 0) w.cut = cut;
-    return;
-  }
-  Held<kChunkThreads> held(w);
-  const uint32_t listed = w.listed;
-  Needed need{w.k_step, w.p_low, w.p_high, w.k_before, listed != kUnlisted};
-  if (need.listed)
-    for (int i = tid; i < (int)listed; i += kChunkThreads) list[i] = w.list[i];
-  const Row r(s, row, red, redf);
-  if (r.greedy) return;  // (no later launch reads its cut)
-  const T* x = row_of<T>(s.a, row);
-  held.scan(red);
-
-  // The (T, n) of a rank among the listed tokens of one step (`above` in front of them) or the whole row (step < 0), by
-  // counts (the first `limit`) or by weight within `in` (tokens before which the weight is below `goal`): radix steps
-  // of up to 11 bits of the key from the highest bit in which the candidates differ, each a histogram scanned
-  // from its largest bucket, until the candidates are equal.
-  auto select = [&](int step, u64 above, bool by_weight, u64 limit, double goal, Cut in) {
-    const int n = step < 0 ? vocab : (int)listed;
-    int known = 32;  // candidates: key >> known == prefix
-    uint32_t prefix = 0;
-    auto candidate = [&](int i, uint32_t& key) {
-      key = step < 0 ? order_key(logit_at(x, i)) : list[i];
-      if (known < 32 && (key >> known) != prefix) return false;
-      if (by_weight && key <= in.key) return false;
-      return step < 0 || r.step(logit_of_key(key)) == step;
-    };
-    const bool extra = by_weight && in.ties != 0;  // the cut's own tokens count as in.ties of them
-    for (;;) {
-      for (int i = tid; i < kBuckets; i += kChunkThreads) hist[i] = 0, count[i] = 0;
-      if (tid == 0) differ = 0u, sample_key = 0u, pick_step = 0xFFFFFFFFu;
-      __syncthreads();
-      const bool extra_now = extra && (known == 32 || (in.key >> known) == prefix);
-      uint32_t key, mine = 0, lo = 0xFFFFFFFFu;
-      for (int i = tid; i < n; i += kChunkThreads)
-        if (candidate(i, key)) mine = max(mine, key), lo = min(lo, key);
-      if (extra_now && tid == 0) mine = max(mine, in.key), lo = min(lo, in.key);
-      if (mine) atomicMax(&sample_key, mine);
-      __syncthreads();
-      const uint32_t top = sample_key;  // the largest candidate
-      if (top == 0u) return in;
-      if (mine && (lo ^ top) != 0u) atomicMax(&differ, lo ^ top);  // its highest bit: the highest that differs
-      __syncthreads();
-      const uint32_t bits_off = differ;
-      const int hb = bits_off ? 31 - __clz((int)bits_off) : -1, shift = max(0, hb - 10), bits = hb + 1 - shift;
-      const uint32_t mask = bits ? (1u << bits) - 1u : 0u;
-      for (int i = tid; i < n; i += kChunkThreads) {
-        if (!candidate(i, key)) continue;
-        const uint32_t bucket = (key >> shift) & mask;
-        atomicAdd(&count[bucket], 1u);
-        if (by_weight) atomicAdd(&hist[bucket], r.fixed(logit_of_key(key)));
-      }
-      __syncthreads();
-      if (extra_now && tid == 0) {
-        const uint32_t bucket = (in.key >> shift) & mask;
-        count[bucket] += in.ties;
-        hist[bucket] += in.ties * r.fixed(logit_of_key(in.key));
-      }
-      __syncthreads();
-      if (hb < 0) {  // all equal (bucket 0)
-        const u64 have = count[0];
-        Cut c{top, 0};
-        if (!by_weight) {
-          c.ties = (uint32_t)min(have, limit - above);
-        } else {
-          const u64 one = r.fixed(logit_of_key(top));
-          u64 j = 1;  // the first tie has less than `goal` before it
-          const double guess = (goal - (double)above) / (double)one;
-          if (guess > 2.0) j = guess < (double)have ? (u64)guess - 1u : have;
-          while (j > 1 && !((double)(above + (j - 1) * one) < goal)) --j;
-          while (j < have && (double)(above + j * one) < goal) ++j;
-          c.ties = (uint32_t)j;
-        }
-        return c;
-      }
-      // this thread's adjacent buckets, the largest first; the smallest non-empty one that starts within the rank
-      constexpr int kPer = kBuckets / kChunkThreads;
-      const int hi = kBuckets - 1 - kPer * tid;
-      u64 b[kPer], sum = 0, total, my_before = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) b[i] = by_weight ? hist[hi - i] : count[hi - i], sum += b[i];
-      u64 run = above + block_scan<kChunkThreads>(sum, red, total);
-      uint32_t my = 0xFFFFFFFFu;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (b[i] && (by_weight ? (double)run < goal : run < limit)) my = hi - i, my_before = run;
-        run += b[i];
-      }
-      if (my != 0xFFFFFFFFu) atomicMin(&pick_step, my);
-      __syncthreads();
-      const uint32_t got = pick_step;
-      if (got == 0xFFFFFFFFu) return in;
-      if (got == my) pick[0] = my_before;
-      __syncthreads();
-      above = pick[0];
-      prefix = shift + bits < 32 ? ((top >> (shift + bits)) << bits) | got : got;
-      known = shift;
-      __syncthreads();
-    }
-  };
-
-  if (need.k_step >= 0)
-    cut = need.listed ? select(need.k_step, need.k_before, false, (u64)k, 0.0, cut) : select(-1, 0, false, (u64)k, 0.0, cut);
-  if (top_p) {
-    // weight of what is kept so far: whole steps, and the kept part of the cut one
-    const int last = need.k_step < 0 ? kBuckets : need.k_step;
-    u64 total = held.weight_to(last, pick), last_weight = 0;
-    if (need.k_step >= 0) {
-      u64 part = 0;
-      const int n = need.listed ? (int)listed : vocab;
-      for (int i = tid; i < n; i += kChunkThreads) {
-        const uint32_t key = need.listed ? list[i] : order_key(logit_at(x, i));
-        const float v = logit_of_key(key);
-        if (key > cut.key && r.step(v) == last) part += r.fixed(v);
-      }
-      if (tid == 0) part += cut.ties * r.fixed(logit_of_key(cut.key));
-      block_scan<kChunkThreads>(part, red, last_weight);
-    }
-    total += last_weight;
-    const double goal = (double)p * (double)total;
-    if (!(goal > 0.0)) {
-      cut = Cut{r.top_key, 1u};
-    } else if (!need.listed) {
-      cut = select(-1, 0, true, 0, goal, cut);
-    } else {
-      const auto f = held.find(true, 0, goal, last, last_weight, pick, &pick_step);
-      cut = select(f.step, f.before, true, 0, goal, f.step == last ? cut : Cut{0u, 0u});
-    }
-  }
-  if (tid == 0) w.cut = cut;
 }
 
 // The kept weight of a logit, without regard to ties.
@@ -541,17 +432,217 @@ __device__ __forceinline__ double least_weight(const Sampler& s, int row) {
   return q > 0.0f ? (double)fminf(q, 1.0f) * (double)(1ull << s.unit_bits) : 0.0;
 }
 
+// The cuts of one row, and its draw where the list holds all that is kept: grid = rows.
+template <class T>
+__global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
+  __shared__ u64 hist[kBuckets];
+  __shared__ uint32_t count[kBuckets];
+  __shared__ u64 list[kList], list_weight[kList];
+  __shared__ u64 red[kRed], pick[4];
+  __shared__ uint32_t pick_step, differ, sample_key;
+  const int row = blockIdx.x, tid = threadIdx.x, vocab = s.a.vocab;
+  Cut cut{0u, 0u};  // everything: every key is above 0 (-inf has key 0x007FFFFF)
+  int k;
+  float p;
+  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
+  RowSpace& w = s.space[row];
+  if (!top_k && !top_p) {
+    if (tid == 0) w.cut = cut, w.drawn = 0;
+    return;
+  }
+  const uint32_t listed = w.listed;
+  Needed need{w.k_step, w.p_low, w.p_high, w.k_before, listed != kUnlisted};
+  const bool small = small_k(top_k, k);
+  const float uf = s.a.uniforms[row];
+  const double least = least_weight(s, row);
+  Held<kChunkThreads> held(w);
+  if (need.listed)
+    for (int i = tid; i < (int)listed; i += kChunkThreads) list[i] = w.list[i];
+  const Row r(s, row, red);
+  if (r.greedy) {
+    if (tid == 0) s.a.token_ids[row] = r.top_index, w.drawn = 1;
+    return;
+  }
+  const T* x = row_of<T>(s.a, row);
+  if (!small) held.scan(red);
+  if (top_p && need.listed)  // (each thread the entries that it has copied)
+    for (int i = tid; i < (int)listed; i += kChunkThreads) list_weight[i] = r.fixed(logit_of_key((uint32_t)(list[i] >> 32)));
+
+  // Selects in falling order of 32-bit keys among candidates get(i, key), i < n, plus extra.ties more at extra.key, with
+  // `above` in front of them: the key T at which a rank ends and the number of candidates at T within it.  The
+  // rank takes candidates before which there are fewer than `limit` (kCount), or weight below `goal` (kBelow), or
+  // not above it (kUpTo).  Radix steps of up to 11 bits from the highest bit in which the candidates differ, each a
+  // histogram scanned from its largest bucket, until the candidates are equal.
+  enum { kCount, kBelow, kUpTo };
+  auto select = [&](int n, auto get, auto weight, u64 above, int rank, u64 limit, double goal, Cut extra, Cut none) {
+    int known = 32;  // candidates: key >> known == prefix
+    uint32_t prefix = 0;
+    auto candidate = [&](int i, uint32_t& key) { return get(i, key) && (known == 32 || (key >> known) == prefix); };
+    auto within = [&](u64 v) { return rank == kCount ? v < limit : rank == kBelow ? (double)v < goal : !((double)v > goal); };
+    for (;;) {
+      for (int i = tid; i < kBuckets; i += kChunkThreads) hist[i] = 0, count[i] = 0;
+      if (tid == 0) differ = 0u, sample_key = 0u, pick_step = 0xFFFFFFFFu;
+      __syncthreads();
+      const bool extra_now = extra.ties && (known == 32 || (extra.key >> known) == prefix);
+      uint32_t key, mine = 0, lo = 0xFFFFFFFFu;
+      for (int i = tid; i < n; i += kChunkThreads)
+        if (candidate(i, key)) mine = max(mine, key), lo = min(lo, key);
+      if (extra_now && tid == 0) mine = max(mine, extra.key), lo = min(lo, extra.key);
+      if (mine) atomicMax(&sample_key, mine);
+      __syncthreads();
+      const uint32_t top = sample_key;  // the largest candidate
+      if (top == 0u) return none;
+      if (mine && (lo ^ top) != 0u) atomicMax(&differ, lo ^ top);  // its highest bit: the highest that differs
+      __syncthreads();
+      const uint32_t bits_off = differ;
+      const int hb = bits_off ? 31 - __clz((int)bits_off) : -1, shift = max(0, hb - 10), bits = hb + 1 - shift;
+      const uint32_t mask = bits ? (1u << bits) - 1u : 0u;
+      for (int i = tid; i < n; i += kChunkThreads) {
+        if (!candidate(i, key)) continue;
+        const uint32_t bucket = (key >> shift) & mask;
+        atomicAdd(&count[bucket], 1u);
+        if (rank != kCount) atomicAdd(&hist[bucket], weight(i, key));
+      }
+      __syncthreads();
+      if (extra_now && tid == 0) {
+        const uint32_t bucket = (extra.key >> shift) & mask;
+        count[bucket] += extra.ties;
+        hist[bucket] += extra.ties * r.fixed(logit_of_key(extra.key));
+      }
+      __syncthreads();
+      if (hb < 0) {  // all equal (bucket 0)
+        const u64 have = count[0], one = rank == kCount ? 0ull : hist[0] / have;
+        Cut c{top, 1};
+        if (rank == kCount) {
+          c.ties = (uint32_t)min(have, limit - above);
+        } else {
+          u64 j = 1;  // the first one is within the rank
+          const double guess = (goal - (double)above) / (double)one;
+          if (guess > 2.0) j = guess < (double)have ? (u64)guess - 1u : have;
+          while (j > 1 && !within(above + (j - 1) * one)) --j;
+          while (j < have && within(above + j * one)) ++j;
+          c.ties = (uint32_t)j;
+        }
+        __syncthreads();
+        return c;
+      }
+      // this thread's adjacent buckets, the largest first; the smallest non-empty one that starts within the rank
+      constexpr int kPer = kBuckets / kChunkThreads;
+      const int hi = kBuckets - 1 - kPer * tid;
+      u64 b[kPer], sum = 0, total, my_before = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) b[i] = rank == kCount ? count[hi - i] : hist[hi - i], sum += b[i];
+      u64 run = above + block_scan<kChunkThreads>(sum, red, total);
+      uint32_t my = 0xFFFFFFFFu;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (b[i] && within(run)) my = hi - i, my_before = run;
+        run += b[i];
+      }
+      if (my != 0xFFFFFFFFu) atomicMin(&pick_step, my);
+      __syncthreads();
+      const uint32_t got = pick_step;
+      if (got == 0xFFFFFFFFu) return none;
+      if (got == my) pick[0] = my_before;
+      __syncthreads();
+      above = pick[0];
+      prefix = shift + bits < 32 ? ((top >> (shift + bits)) << bits) | got : got;
+      known = shift;
+      __syncthreads();
+    }
+  };
+  auto key_weight = [&](int i, uint32_t key) { return need.listed ? list_weight[i] : r.fixed(logit_of_key(key)); };
+  auto list_key = [&](int i) { return (uint32_t)(list[i] >> 32); };
+  // by counts: the first k of the tokens of the cut's step (the whole row without a list)
+  auto top_k_cut = [&]() {
+    const int step = need.k_step;
+    if (need.listed)
+      return select((int)listed, [&](int i, uint32_t& key) { key = list_key(i); return r.step(logit_of_key(key)) == step; },
+                    key_weight, need.k_before, kCount, (u64)k, 0.0, Cut{0u, 0u}, cut);
+    return select(vocab, [&](int i, uint32_t& key) { key = order_key(logit_at(x, i)); return true; }, key_weight, 0, kCount,
+                  (u64)k, 0.0, Cut{0u, 0u}, cut);
+  };
+  // by weight: what is below `goal` of the tokens within `in` of a step (step < 0: of all listed, of the row without a list)
+  auto top_p_cut = [&](int step, u64 before, double goal, Cut in) {
+    if (need.listed)
+      return select((int)listed, [&](int i, uint32_t& key) {
+        key = list_key(i);
+        return key > in.key && (step < 0 || r.step(logit_of_key(key)) == step);
+      }, key_weight, before, kBelow, 0, goal, in, in);
+    return select(vocab, [&](int i, uint32_t& key) { key = order_key(logit_at(x, i)); return key > in.key; }, key_weight, 0,
+                  kBelow, 0, goal, in, in);
+  };
+  // weight of the listed tokens (of the row without a list) above the cut in a step (< 0: in all), and of its ties
+  auto weight_of = [&](int step) {
+    u64 part = 0, total;
+    const int n = need.listed ? (int)listed : vocab;
+    for (int i = tid; i < n; i += kChunkThreads) {
+      const uint32_t key = need.listed ? list_key(i) : order_key(logit_at(x, i));
+      if (key > cut.key && (step < 0 || r.step(logit_of_key(key)) == step)) part += key_weight(i, key);
+    }
+    if (tid == 0 && cut.ties) part += cut.ties * r.fixed(logit_of_key(cut.key));
+    block_scan<kChunkThreads>(part, red, total);
+    return total;
+  };
+
+  __syncthreads();
+  if (need.k_step >= 0) cut = top_k_cut();
+  if (top_p) {
+    // weight of what is kept so far: whole steps, and the kept part of the cut one
+    const int last = need.k_step < 0 ? kBuckets : need.k_step;
+    u64 total, last_weight = 0;
+    if (small || !need.listed) {
+      total = weight_of(-1);
+    } else {
+      total = held.weight_to(last, pick);
+      if (need.k_step >= 0) last_weight = weight_of(last);
+      total += last_weight;
+    }
+    const double goal = (double)p * (double)total;
+    if (!(goal > 0.0)) {
+      cut = Cut{r.top_key, 1u};
+    } else if (small || !need.listed) {
+      cut = top_p_cut(-1, 0, goal, cut);
+    } else {
+      const auto f = held.find(true, 0, goal, last, last_weight, pick, &pick_step);
+      cut = top_p_cut(f.step, f.before, goal, f.step == last ? cut : Cut{0u, 0u});
+    }
+  }
+  if (!small || !need.listed) {
+    if (tid == 0) w.cut = cut, w.drawn = 0;
+    return;
+  }
+  // The draw from the list: the last index (in rising order: the falling one of ~index) of the ties that are kept, then the
+  // index at which the running weight passes the goal
+  const u64 tie = cut.ties ? kept_weight(r, logit_of_key(cut.key), least) : 0ull;
+  const Cut end = cut.ties ? select((int)listed, [&](int i, uint32_t& key) { key = ~(uint32_t)list[i]; return list_key(i) == cut.key; },
+                                    key_weight, 0, kCount, cut.ties, 0.0, Cut{0u, 0u}, Cut{0u, 0u})
+                           : Cut{0xFFFFFFFFu, 0u};
+  u64 sum = 0, total;
+  for (int i = tid; i < (int)listed; i += kChunkThreads) {
+    const uint32_t key = list_key(i);
+    list_weight[i] = key > cut.key ? kept_weight(r, logit_of_key(key), least)
+                                   : key == cut.key && ~(uint32_t)list[i] >= end.key ? tie : 0ull;
+    sum += list_weight[i];
+  }
+  block_scan<kChunkThreads>(sum, red, total);
+  const double goal = (uf > 0.0f ? (double)fminf(uf, 1.0f) : 0.0) * (double)total;
+  const Cut token = select((int)listed, [&](int i, uint32_t& key) { key = ~(uint32_t)list[i]; return list_weight[i] != 0; },
+                           key_weight, 0, kUpTo, 0, goal, Cut{0u, 0u}, Cut{~(uint32_t)r.top_index, 0u});
+  if (tid == 0) s.a.token_ids[row] = (int)~token.key, w.drawn = 1;
+}
+
 // Kept weight above the cut, and number of tokens at it, of each segment: a wave per segment, in turn.
 // grid = (blocks, rows).
 template <class T>
 __global__ void __launch_bounds__(kChunkThreads) sample_segment_kernel(Sampler s) {
-  __shared__ u64 red[kChunkThreads / 64];
-  __shared__ float redf[kChunkThreads / 64];
+  __shared__ u64 red[kRed];
   const int row = blockIdx.y, lane = threadIdx.x & 63;
   const T* x = row_of<T>(s.a, row);
+  if (s.space[row].drawn) return;
   const Cut cut = s.space[row].cut;
   const double least = least_weight(s, row);
-  const Row r(s, row, red, redf);
+  const Row r(s, row, red);
   if (r.greedy) return;
   for (int seg = blockIdx.x * (kChunkThreads / 64) + (threadIdx.x >> 6); seg < s.segments; seg += gridDim.x * (kChunkThreads / 64)) {
     u64 w = 0;
@@ -568,11 +659,8 @@ __global__ void __launch_bounds__(kChunkThreads) sample_segment_kernel(Sampler s
         if (key == cut.key && i0 + 64 * j < s.a.vocab) ++n;
       }
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      w += __shfl_xor(w, off, 64);
-      n += __shfl_xor(n, off, 64);
-    }
+    w = wave_sum(w);
+    n = wave_sum(n);
     if (lane == 0) {
       s.seg_weight[(size_t)row * s.segments + seg] = w;
       s.seg_ties[(size_t)row * s.segments + seg] = n;
@@ -583,11 +671,11 @@ __global__ void __launch_bounds__(kChunkThreads) sample_segment_kernel(Sampler s
 // The draw: the segment that holds the goal, then the token in it.  One segment a thread; grid = rows.
 template <class T>
 __global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
-  __shared__ u64 red[kThreads / 64];
-  __shared__ float redf[kThreads / 64];
+  __shared__ u64 red[kRed];
   __shared__ u64 pick_above;
   __shared__ uint32_t pick_segment, pick_seen;
   const int row = blockIdx.x, tid = threadIdx.x;
+  if (s.space[row].drawn) return;
   // everything that the row's weights do not decide, before the first wait
   const bool live = tid < s.segments;
   const u64 my_weight = live ? s.seg_weight[(size_t)row * s.segments + tid] : 0ull;
@@ -595,7 +683,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
   const Cut cut = s.space[row].cut;
   const double least = least_weight(s, row);
   const float uf = s.a.uniforms[row];
-  const Row r(s, row, red, redf);
+  const Row r(s, row, red);
   if (r.greedy) {
     if (tid == 0) s.a.token_ids[row] = r.top_index;
     return;
@@ -630,13 +718,8 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
     uint32_t held = 0;
 #pragma unroll
     for (int j = 0; j < kLane; ++j) held += first + j < s.a.vocab && order_key(v[j]) == cut.key ? 1u : 0u;
-    uint32_t rank = held;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = __shfl_up(rank, off, 64);
-      if (tid >= off) rank += o;
-    }
-    const uint32_t rank_next = rank0 + __shfl(rank, 63, 64);
+    uint32_t rank = wave_scan(held);
+    const uint32_t rank_next = rank0 + last_lane(rank);
     rank += rank0 - held;
     u64 here[kLane], sum = 0;
 #pragma unroll
@@ -646,13 +729,8 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
       if (first + j < s.a.vocab && key == cut.key && rank++ < cut.ties) here[j] = tie;
       sum += here[j];
     }
-    u64 run = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const u64 o = __shfl_up(run, off, 64);
-      if (tid >= off) run += o;
-    }
-    const u64 above_next = above + __shfl(run, 63, 64);
+    u64 run = wave_scan(sum);
+    const u64 above_next = above + last_lane(run);
     run += above - sum;
     int past = -1, some = -1;  // the lane's first token beyond the goal, and its last one with weight
 #pragma unroll

@@ -13,6 +13,11 @@ namespace qwen {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// Probabilities enter the products times 2^11 relative to a maximum that may lag the true one by a factor of 2^4 (so that
+// the accumulators are rescaled rarely): up to 2^15, and normal in fp16 down to 2^-25 of the largest.
+constexpr float kProbBits = 11.0f, kProbLag = 4.0f;
 
 struct Bf16 {  // storage of a bf16 element
   uint16_t bits;
