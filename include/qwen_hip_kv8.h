@@ -70,7 +70,7 @@ typedef struct qwen_kv8_rows {
 /* Stores `rows` new tokens of sequences 0..batch-1: row i of sequence b becomes token positions[b] + i.
  * positions [batch] int32: each sequence's past length.  Sequences with a negative position are left as
  * they are (inactive slots of a padded batch), and so are tokens at or behind 64 * blocks (dropped).
- * Codes behind the last new token keep their bytes. */
+ * Codes behind the last new token keep their bytes.  batch 1 .. 65535, rows 1 .. 2^24 (in all calls). */
 int qwen_hip_kv8_store(const qwen_kv8_cache* cache, int type, const qwen_kv8_rows* k, const qwen_kv8_rows* v, int batch,
                        int rows, const int* positions, void* stream);
 
@@ -97,6 +97,7 @@ int qwen_hip_kv8_attention_workspace(const qwen_kv8_cache* cache, int type, int 
  * bits) and so do the probabilities; QWEN_TYPE_BF16 queries and their probabilities as one.  The codes are
  * exact in fp16.  A query without a token to attend (a negative position) gives zeros.
  *   q_heads    a multiple of kv_heads, at most 64 query heads a KV head
+ *   rows       rows * q_heads / kv_heads and batch * kv_heads: at most 2^22 each
  *   max_keys   host int >= max(positions) + rows, at most 64 * blocks (sizes the split over the keys); tokens
  *              at or behind it are not attended
  *   workspace  16-byte aligned, qwen_hip_kv8_attention_workspace bytes; contents need not be kept

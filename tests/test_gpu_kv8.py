@@ -277,6 +277,32 @@ def test_attend_ignores_what_lies_behind(torch):
     assert np.isfinite(cut).all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sequences,blocks,dim", [(15, 25, 64), (15, 25, 128), (80, 25, 64), (80, 25, 128), (40, 80, 64)])
+def test_attend_large_tiles(torch, dtype, sequences, blocks, dim):
+    """Tiles of many rows, split over the keys or not, with one key group a workgroup (15 sequences) or several: ragged
+    lengths, V scales far apart, NaN scales behind a sequence and in the reach of its last rows only."""
+    rows, rng = 17, np.random.default_rng(blocks + dim)
+    cache = filled(torch, sequences, blocks, 2, dim, sequences + blocks)
+    cache.v_scale[0] *= torch.exp2(torch.from_numpy(rng.choice([0.0, 0.0, -1.0, -7.0, 9.0, -30.0], (sequences, blocks, 2))).float()).cuda()
+    end = 64 * blocks - rows
+    positions = [[-1, 0, 1, 47, 48, 63, 64, 600, 1000, end - 64, end - 1, end][b % 12] for b in range(sequences)]
+    for b, pos in enumerate(positions):
+        last = (pos + rows - 1) // 64  # block of the last row
+        if b % 2 and pos >= 0:
+            cache.k_scale[0, b, last + 1:] = float("nan")
+            cache.v_scale[0, b, last + 1:] = float("nan")
+        elif b % 4 == 0 and pos // 64 < last:
+            (cache.k_scale if b % 8 else cache.v_scale)[0, b, last] = float("nan")
+    q, qn = rows_of(torch, rng, (sequences, rows, 4, dim), dtype, 0.3)
+    want, slack, floor, reach = Cache.of(cache).attend(qn, positions, 0.1)
+    got = cache.attend(0, q, ints(torch, positions), 64 * blocks, scale=0.1).float().cpu().numpy()
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    assert np.isnan(want).any() and not np.isnan(want).all(axis=(1, 2, 3)).any()
+    tol = tolerance("f32" if dtype == "float32" else "bf16", dim, slack, floor, reach, want)
+    assert (np.abs(got - want) <= tol)[~np.isnan(want)].all()
+
+
 def test_attend_non_finite_queries(torch):
     cache = filled(torch, 1, 2, 1, 64, 14)
     q = torch.ones(1, 4, 1, 64, device="cuda")

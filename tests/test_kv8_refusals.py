@@ -66,7 +66,8 @@ def test_kv8_refuses_overlapping_results(lib, op, which, over):
 
 @pytest.mark.parametrize("bad", [dict(heads=0), dict(heads=3), dict(heads=130), dict(heads=-2), dict(max_keys=0),
                                  dict(max_keys=513), dict(max_keys=-1), dict(scale=float("nan")),
-                                 dict(scale=float("inf")), dict(c=cache(blocks=64), max_keys=4096, ws=None),
+                                 dict(scale=float("inf")), dict(scale=3e38), dict(n=(1 << 21) + 1),
+                                 dict(c=cache(sequences=65535, kv_heads=128), batch=65535, heads=128), dict(c=cache(blocks=64), max_keys=4096, ws=None),
                                  dict(c=cache(blocks=64), max_keys=4096, ws_bytes=16),
                                  dict(c=cache(blocks=64), max_keys=4096, ws=PTR + 4)])
 def test_kv8_attention_refuses(lib, bad):

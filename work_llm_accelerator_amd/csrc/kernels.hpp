@@ -298,6 +298,7 @@ void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, 
 // cache blocks, joined by a second launch through `workspace` bytes where nsplit > 1.
 struct Kv8AttnPlan {
   int tiles, tile_rows, groups, nsplit, per_split;
+  bool one_key_group;  // of the kernel of large tiles
   size_t workspace;
 };
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys);

@@ -32,7 +32,9 @@ __device__ __forceinline__ uint32_t regrade(uint32_t w, float ratio) {
 // One block of 256 threads per (64-token cache block, head, K or V, sequence): the block's new rows are read once
 // into registers, their largest magnitude gives the scale (a maximum of bit patterns: non-finite values come
 // out on top), and the codes are written once; V goes through LDS to turn 4 x 4 bytes.  The earlier rows of a
-// part-filled block are read only where the scale grows.  Bound by the stream of new rows.
+// part-filled block are read only where the scale grows.  Bound by the stream of new rows: 8 x 2048 tokens (bf16, 2 heads
+// of 128) 8.4 us for 50 MB, out of the caches; single tokens by the launch and two round trips to memory: 4.8 us for one
+// sequence, 5.6 for 64.
 // grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv8_store_kernel(qwen_kv8_cache c, qwen_kv8_rows kin, qwen_kv8_rows vin, int rows,
@@ -177,7 +179,9 @@ __global__ void __launch_bounds__(256) fill_i32_kernel(int* __restrict__ p, int 
 }
 
 // ---- load -----------------------------------------------------------------------------------
-// The inverse, one block of 256 threads per (cache block, head, K or V, sequence); bound by the rows written.
+// The inverse, one block of 256 threads per (cache block, head, K or V, sequence); bound by the rows written: 4 x 32768
+// tokens (bf16, 2 heads of 128) 72 us for 336 MB, 4.7 TB/s where a copy reaches 5.2; with 8-byte stores 80 us, with
+// nontemporal ones 76 or 116 from run to run.
 // grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv8_load_kernel(qwen_kv8_cache c, qwen_kv8_rows kout, qwen_kv8_rows vout, int rows,
@@ -271,8 +275,10 @@ __device__ __forceinline__ uint4 load_once(const int8_t* p) {
 //   joined in LDS.
 // fp32 queries take two columns each (hi and lo fp16 terms, 8 apart), whose scores are added across lanes; the
 // columns then carry the hi and lo terms of the probabilities.
-// grid = (nsplit * tile groups, kv_heads, batch), block = 256 (with 512 threads, eight waves a block: 64 x 4096 1 us more, one sequence of 578
-// tokens 0.2 us more).
+// Bound by HBM: 64 sequences of 4096 tokens (fp32, 12 / 2 heads of 128) 25.1 us, of which 135 MB take 18 at 7.4 TB/s
+// and the rest is ramp, join and the last blocks; one sequence of 578 tokens 8.6 us, latency alone.
+// grid = (nsplit * tile groups, kv_heads, batch), block = 256 (with 512 threads, eight waves a block: 64 x 4096 1 us
+// more, one sequence of 578 tokens 0.2 us more).
 template <class T, int D, int CT>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) kv8_attn_kernel(Kv8AttnArgs a) {
   constexpr bool kTwo = std::is_same<T, float>::value;
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) k
       if constexpr (kTwo) y += join[w][ct][dt][16 * q4 + c + 8] * f;
     }
     const int dim = 16 * dt + 4 * q4;
-    if (a.nsplit > 1) {
+    if (nblk > a.per_split) {  // (else the only live split)
       const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit + split;
       if (dim == 0) a.pml[at] = make_float2(mm, total);
       store4(a.part + at * D + dim, y);
@@ -492,7 +498,11 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) k
 }
 
 // Joins the key splits of a query row: D / 4 lanes hold four dimensions each.  With many splits a block has one row
-// and divides the splits over its lane groups; with few it has a row per lane group.
+// and divides the splits over its lane groups; with few it has a row per lane group (12 rows of 125 splits: 4.7 us and 16;
+// 3600 rows of 12 splits: 7.2 and 5.2).
+constexpr int kMergeWide = 16;
+// A row whose tile has one live split is in the output already.  64 x 4096 of 12 heads, two splits each: 4.2 us, most of
+// it the launch.
 // grid = (rows * group / rows of a block, kv_heads, batch), block = 256.
 template <class T, int D, bool kMany>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(Kv8AttnArgs a) {
@@ -505,6 +515,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(Kv8AttnArgs a) {
   const int i_last = min(R - 1, row / a.tile_rows * a.tile_rows + a.tile_rows - 1) / a.group;
   const int kmax = pos < 0 ? 0 : (int)min((long long)pos + i_last + 1, (long long)a.max_keys);
   const int live = ((kmax + kKv8Block - 1) / kKv8Block + a.per_split - 1) / a.per_split;
+  if (live == 1) return;  // already in the output
   const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit;
   const f32x4* part = reinterpret_cast<const f32x4*>(a.part + at * D) + lane;
   float m = -__builtin_inff(), sum = 0.0f;
@@ -551,9 +562,9 @@ void run_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int batch, hipStream_t
   else if (p.tiles == 2)
     hipLaunchKernelGGL((kv8_attn_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
   else
-    launch_kv8_attention_tiles(a, std::is_same<T, float>::value ? QWEN_TYPE_F32 : QWEN_TYPE_BF16, batch, p.groups, st);
+    launch_kv8_attention_tiles(a, std::is_same<T, float>::value ? QWEN_TYPE_F32 : QWEN_TYPE_BF16, batch, p.groups, p.one_key_group, st);
   const int R = a.rows * a.group, per_block = 1024 / D;
-  if (a.nsplit > 4)
+  if (a.nsplit > kMergeWide)
     hipLaunchKernelGGL((kv8_merge_kernel<T, D, true>), dim3(R, a.c.kv_heads, batch), dim3(256), 0, st, a);
   else if (a.nsplit > 1)
     hipLaunchKernelGGL((kv8_merge_kernel<T, D, false>), dim3((R + per_block - 1) / per_block, a.c.kv_heads, batch), dim3(256), 0, st, a);
@@ -603,6 +614,15 @@ void launch_fill_i32(int* p, int n, int value, hipStream_t st) {
   hipLaunchKernelGGL(fill_i32_kernel, dim3((n + 255) / 256), dim3(256), 0, st, p, n, value);
 }
 
+// Rows and keys over the workgroups; bf16 in parentheses where both types were timed.
+// - More than two tiles of 16 columns go to the kernel of large tiles.
+// - Keys are split to one workgroup a CU (512, 768 or 1024 of them: slower, by their joins), in whole turns of the four
+//   waves.  A sequence of up to 12 blocks is not split: three blocks a wave cost less than the second launch.
+// - From 160 large tiles on, no split: the parts of many rows cost more than the CUs left idle (28 tiles of 1701 keys times
+//   8 heads, head_dim 64: 38 us (30) whole, 42 (36) split; 192 tiles of 2560 keys: 79 us (53), 81 (63)).
+// - Three key groups a workgroup where it has 24 blocks or more and the workgroups are less than two a CU (384 tiles of 64
+//   blocks: 129 us (84), one key group 158 (108)), else one (384 tiles of 8 blocks: 37 us (33), 31 (22); 768 of 64:
+//   229 us (152), 206 (140)).
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys) {
   const bool two = type == QWEN_TYPE_F32;
   const long long R = (long long)rows * (q_heads / c.kv_heads);
@@ -621,6 +641,7 @@ Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, i
   per = (per + 3) / 4 * 4;
   p.per_split = (int)per;
   p.nsplit = (int)((blocks + per - 1) / per);
+  p.one_key_group = per < 24 || others * p.nsplit >= 512;
   if (p.nsplit > 1)
     p.workspace = (size_t)batch * q_heads * rows * p.nsplit * (size_t)(c.head_dim + 2) * sizeof(float);
   return p;

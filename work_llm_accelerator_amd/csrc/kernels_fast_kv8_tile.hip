@@ -1,13 +1,18 @@
 // Attention of many query rows (prompts, chunks) over the 8-bit K/V cache: tiles of 128 rows.
 //
 // kv8_attn_kernel feeds each wave its own cache blocks from HBM and converts their codes for 32 columns at most; here the
-// work is bound by the softmax's vector instructions and the matrix cores, so codes are converted once for the
-// whole tile and shared through LDS.  A block has eight waves: four column groups of 32 rows times two key groups,
-// which take the 64-token cache blocks in turn and are joined at the end.  The two waves of a SIMD are of
-// different key groups and half a turn apart: while one has the matrix cores (O^T += V P^T of its last block,
-// S^T = K Q^T of its next, 32x32x16 fp16), the other has the vector instructions (the softmax, a lane holding one
-// column and half of the tokens, and the conversion of its group's next codes).  A barrier ends each half turn, so
-// K and V need one LDS buffer a group each.
+// work is bound by the softmax's vector instructions and the LDS reads of the products, so the codes of a 64-token cache
+// block are converted once for the whole tile and shared through LDS.  Four waves of 32 columns are a key group
+// (S^T = K Q^T and O^T += V P^T, 32x32x16 fp16; a lane holds one column and half of the block's tokens).
+//
+// One key group a workgroup (KG = 1), 256 registers a wave and so two workgroups a CU, which drift half a turn apart by
+// themselves: while one has the matrix cores, the other has the vector instructions.  Four causal prompts of 4096
+// tokens (12 / 2 heads of 128, bf16): 253 us = 815 TFLOP/s, 74 % of a large library product's rate here; with three
+// key groups 287.  fp32: 390 us, 530.
+// Where the tiles of a call are too few for that and each has many blocks, its longest tile decides: then two or three key
+// groups of a workgroup (KG) take the blocks in turn, kept a part of a turn apart by barriers, and are joined at the
+// end.  One such prompt: 83 us, with KG = 1 96 to 108 (also as two splits, or as tiles of 64 rows with two key groups
+// of two waves: 98).
 // fp32 rows enter as hi and lo fp16 terms in two products each, as their probabilities do.
 #include "kv8_device.hpp"
 
@@ -28,24 +33,25 @@ __device__ __forceinline__ float swap_sum(float x) {
   return bits_f32(r[0]) + bits_f32(r[1]);
 }
 
-// grid = (nsplit * tiles, kv_heads, batch), block = 256 * KG.
+// grid = (kv_heads * batch, tiles, nsplit), block = 256 * KG.  Blocks start in the order of their number: the tiles with the
+// longest rows of all heads and sequences first.  Heads rotate from one row of the grid to the next, or those of a long
+// sequence would all come to the same XCD.
 template <class T, int D, int KG>
-__global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) {
+__global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(KG == 1 ? 2 : KG))) kv8_attn_tile_kernel(Kv8AttnArgs a) {
   constexpr bool kTwo = std::is_same<T, float>::value;
   constexpr int kLimbs = kTwo ? 2 : 1;
   constexpr int kSteps = D / 16, kDims = D / 32, kChunks = D / 8;
   constexpr int kLoads = D / 64;  // 16-byte pieces of K, and pairs of half of them of V, that a thread stages
   __shared__ uint4 kbuf[KG][kKv8Block * kChunks];  // [key group][token][16-byte chunk ^ swizzle]
   __shared__ uint4 vbuf[KG][D * 8];                // [key group][dimension][chunk ^ swizzle]
-  // Query operands: in registers where they take 16, in LDS (the same for all key groups) where they take more
-  constexpr bool kQInLds = kLimbs * kSteps > 4;
+  // Query operands: in registers where there is room, else in LDS (the same for all key groups)
+  constexpr bool kQInLds = kLimbs * kSteps > (KG == 1 ? 16 : 4);
   __shared__ uint4 qbuf[kQInLds ? 4 * kLimbs * kSteps * 64 : 1];  // [column group][term][k step][lane]
-  __shared__ float2 ml[KG - 1][kKv8TileRows];
-  __shared__ int unit_of[KG - 1][kKv8TileRows];
+  __shared__ float2 ml[KG > 1 ? KG - 1 : 1][kKv8TileRows];  // of the key groups after the first
+  __shared__ int unit_of[KG > 1 ? KG - 1 : 1][kKv8TileRows];
 
-  const int tiles = gridDim.x / a.nsplit, split = blockIdx.x % a.nsplit;
-  const int tile = tiles - 1 - (int)(blockIdx.x / a.nsplit);  // the longest rows first
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int tiles = gridDim.y, split = blockIdx.z, tile = tiles - 1 - (int)blockIdx.y;
+  const int head = (blockIdx.x + blockIdx.y + blockIdx.z) % gridDim.x, kvh = head % a.c.kv_heads, b = head / a.c.kv_heads;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cg = wave & 3, kg = wave >> 2;
   const int col = lane & 31, hh = lane >> 5;
   const int R = a.rows * a.group, row0 = tile * kKv8TileRows;
@@ -55,6 +61,7 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
   const int nblk = (kmax + kKv8Block - 1) / kKv8Block;
   const int blk0 = split * a.per_split, blk1 = min(nblk, blk0 + a.per_split);
   if (blk0 >= blk1 && a.nsplit > 1) return;  // the merge knows the live splits
+  const bool parts = nblk > a.per_split;      // more than one: results to be merged
   const int turns = (max(0, blk1 - blk0) + KG - 1) / KG;  // each key group takes every KG-th block
   const int full = min(blk1, kmin / kKv8Block);       // blocks before it need no mask
 
@@ -310,7 +317,7 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
     float sk = a.c.k_scale[place(0)], svf = a.c.v_scale[place(0)];
     __syncthreads();
     // Key group kg runs kg ticks behind.  A barrier counts the waves that arrive, wherever in the code: every wave
-    // comes to KG * (turns + 1) of them.
+    // comes to max(2, KG) * turns + KG of them.
     auto tick = []() {  // (nothing moves across: the work of a tick is balanced)
       __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
   // Join the key groups in LDS, one after the other, and write; accumulators in true units from here on
   f32x4* parked = reinterpret_cast<f32x4*>(kbuf);  // half of the dimensions at a time: [column group][..][quarter][lane]
   constexpr int kPart = kDims / 2;
-  static_assert(sizeof(kbuf) >= sizeof(f32x4) * 4 * kPart * 4 * 64, "the join fits the K buffers");
+  static_assert(KG == 1 || sizeof(kbuf) >= sizeof(f32x4) * 4 * kPart * 4 * 64, "the join fits the K buffers");
   l = swap_sum(l);
   if (kg > 0 && hh == 0) ml[kg - 1][cg * 32 + col] = make_float2(m, l), unit_of[kg - 1][cg * 32 + col] = unit;
   __syncthreads();
@@ -393,15 +400,15 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
   const size_t at = (((size_t)b * a.c.kv_heads + kvh) * R + row) * a.nsplit + split;
   T* dst = static_cast<T*>(a.out.data) + b * a.out.seq_stride + (long long)qi * a.out.token_stride +
            (long long)qh * a.out.head_stride;
-  if (a.nsplit > 1 && hh == 0) a.pml[at] = make_float2(mm, sum_all);
-  const float inv = a.nsplit > 1 ? 1.0f : sum_all == 0.0f ? 0.0f : 1.0f / sum_all;
+  if (parts && hh == 0) a.pml[at] = make_float2(mm, sum_all);
+  const float inv = parts ? 1.0f : sum_all == 0.0f ? 0.0f : 1.0f / sum_all;
 #pragma unroll
   for (int d = 0; d < kDims; ++d)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const f32x4 z = f32x4{o[d][4 * w], o[d][4 * w + 1], o[d][4 * w + 2], o[d][4 * w + 3]} * inv;
       const int dim = 32 * d + 8 * w + 4 * hh;
-      if (a.nsplit > 1)
+      if (parts)
         store4(a.part + at * D + dim, z);
       else
         store4(dst + dim, z);
@@ -410,19 +417,31 @@ __global__ void __launch_bounds__(256 * KG) kv8_attn_tile_kernel(Kv8AttnArgs a) 
 
 }  // namespace
 
-void launch_kv8_attention_tiles(const Kv8AttnArgs& a, int type, int batch, int groups, hipStream_t st) {
-  const dim3 grid(a.nsplit * groups, a.c.kv_heads, batch);
-  if (type == QWEN_TYPE_F32) {
-    if (a.c.head_dim == 64)
-      hipLaunchKernelGGL((kv8_attn_tile_kernel<float, 64, 3>), grid, dim3(768), 0, st, a);
+void launch_kv8_attention_tiles(const Kv8AttnArgs& a, int type, int batch, int groups, bool one_key_group, hipStream_t st) {
+  const dim3 grid(a.c.kv_heads * batch, groups, a.nsplit);
+  auto run = [&](auto t, auto d, auto groups_of_keys) {
+    constexpr int KG = decltype(groups_of_keys)::value;
+    hipLaunchKernelGGL((kv8_attn_tile_kernel<decltype(t), decltype(d)::value, KG>), grid, dim3(256 * KG), 0, st, a);
+  };
+  using One = std::integral_constant<int, 1>;
+  auto by_keys = [&](auto t, auto d) {
+    // three key groups, two where the fp32 queries' LDS leaves no room for more
+    using Some = std::integral_constant<int, std::is_same<decltype(t), float>::value && decltype(d)::value == 128 ? 2 : 3>;
+    if (one_key_group)
+      run(t, d, One{});
     else
-      hipLaunchKernelGGL((kv8_attn_tile_kernel<float, 128, 2>), grid, dim3(512), 0, st, a);
-  } else {
+      run(t, d, Some{});
+  };
+  auto by_dim = [&](auto t) {
     if (a.c.head_dim == 64)
-      hipLaunchKernelGGL((kv8_attn_tile_kernel<Bf16, 64, 3>), grid, dim3(768), 0, st, a);
+      by_keys(t, std::integral_constant<int, 64>{});
     else
-      hipLaunchKernelGGL((kv8_attn_tile_kernel<Bf16, 128, 3>), grid, dim3(768), 0, st, a);
-  }
+      by_keys(t, std::integral_constant<int, 128>{});
+  };
+  if (type == QWEN_TYPE_F32)
+    by_dim(float{});
+  else
+    by_dim(Bf16{});
 }
 
 }  // namespace qwen

@@ -19,6 +19,7 @@ constexpr int kMaxBatch = 65535;       // grid z
 constexpr int kMaxRows = 1 << 24;      // tokens of a call: grids and row counts stay within 32 bits
 constexpr int kMaxHeads = 1024;
 constexpr int kMaxGroup = 64;
+constexpr int64_t kMaxQueryRows = 1 << 22, kMaxHeadRows = 1 << 22;  // of the attention: its grids
 constexpr int64_t kMaxStride = int64_t(1) << 40;
 
 int bad(const char* why) {
@@ -124,6 +125,8 @@ static const char* attention_problem(const qwen_kv8_cache* c, int type, int q_he
   if (q_heads < 1 || q_heads % c->kv_heads != 0 || q_heads / c->kv_heads > kMaxGroup)
     return "q_heads must be a multiple of kv_heads, at most 64 a KV head";
   if (rows < 1 || rows > kMaxRows) return "rows must be 1 .. 2^24";
+  if ((int64_t)rows * (q_heads / c->kv_heads) > kMaxQueryRows) return "rows times query heads a KV head must be at most 2^22";
+  if ((int64_t)batch * c->kv_heads > kMaxHeadRows) return "batch times kv_heads must be at most 2^22";
   if (max_keys < 1 || max_keys > (int64_t)c->blocks * QWEN_KV8_BLOCK) return "max_keys must be 1 .. 64 * blocks";
   return nullptr;
 }
@@ -141,7 +144,7 @@ int qwen_hip_kv8_attention(const qwen_kv8_cache* cache, int type, const qwen_kv8
                            void* workspace, uint64_t workspace_bytes, void* stream) {
   if (const char* why = attention_problem(cache, type, q_heads, batch, rows, max_keys)) return bad(why);
   if (!positions) return bad("null positions");
-  if (!std::isfinite(scale)) return bad("the attention's scale must be finite");
+  if (!std::isfinite(scale * 1.44269504088896340736f)) return bad("the attention's scale must be finite (times log2 e too)");
   if (const char* why = rows_problem(q, type, batch, rows, q_heads, cache->head_dim, false)) return bad(why);
   if (const char* why = rows_problem(out, type, batch, rows, q_heads, cache->head_dim, true)) return bad(why);
   const Kv8AttnPlan plan = plan_kv8_attention(*cache, type, q_heads, batch, rows, max_keys);

@@ -81,6 +81,6 @@ __device__ __forceinline__ half8 codes_to_half(uint32_t lo, uint32_t hi) {
 
 // Attention by tiles of many rows (kernels_fast_kv8_tile.hip): rows of a block, and the launch without a merge.
 constexpr int kKv8TileRows = 128;
-void launch_kv8_attention_tiles(const Kv8AttnArgs& a, int type, int batch, int groups, hipStream_t st);
+void launch_kv8_attention_tiles(const Kv8AttnArgs& a, int type, int batch, int groups, bool one_key_group, hipStream_t st);
 
 }  // namespace qwen
