@@ -293,12 +293,12 @@ void launch_kv8_store(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k,
                       int rows, const int* positions, hipStream_t st);
 void launch_kv8_load(const qwen_kv8_cache& c, int type, const qwen_kv8_rows& k, const qwen_kv8_rows& v, int batch,
                      int rows, bool zero_outside, const int* positions, hipStream_t st);
-// How an attention call is split: the query rows of a sequence and KV head in `groups` groups of tile_rows (tiles: 1 or
-// 2 tiles of 16 columns a wave, or 4: the kernel of large tiles), the keys over nsplit splits of per_split
-// cache blocks, joined by a second launch through `workspace` bytes where nsplit > 1.
+// How an attention call is split: the query rows of a sequence and KV head in `groups` groups of tile_rows (1 or 2
+// tiles of 16 columns, or a large tile with one key group or several), the keys over nsplit splits of per_split cache
+// blocks, joined by a second launch through `workspace` bytes where nsplit > 1.
 struct Kv8AttnPlan {
   int tiles, tile_rows, groups, nsplit, per_split;
-  bool one_key_group;  // of the kernel of large tiles
+  bool large, one_key_group;
   size_t workspace;
 };
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys);

@@ -557,12 +557,12 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(Kv8AttnArgs a) {
 template <class T, int D>
 void run_attn(const Kv8AttnArgs& a, const Kv8AttnPlan& p, int batch, hipStream_t st) {
   const dim3 grid(a.nsplit * p.groups, a.c.kv_heads, batch);
-  if (p.tiles == 1)
-    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 1>), grid, dim3(256), 0, st, a);
-  else if (p.tiles == 2)
-    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
-  else
+  if (p.large)
     launch_kv8_attention_tiles(a, std::is_same<T, float>::value ? QWEN_TYPE_F32 : QWEN_TYPE_BF16, batch, p.groups, p.one_key_group, st);
+  else if (p.tiles == 1)
+    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 1>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv8_attn_kernel<T, D, 2>), grid, dim3(256), 0, st, a);
   const int R = a.rows * a.group, per_block = 1024 / D;
   if (a.nsplit > kMergeWide)
     hipLaunchKernelGGL((kv8_merge_kernel<T, D, true>), dim3(R, a.c.kv_heads, batch), dim3(256), 0, st, a);
@@ -614,34 +614,46 @@ void launch_fill_i32(int* p, int n, int value, hipStream_t st) {
   hipLaunchKernelGGL(fill_i32_kernel, dim3((n + 255) / 256), dim3(256), 0, st, p, n, value);
 }
 
-// Rows and keys over the workgroups; bf16 in parentheses where both types were timed.
-// - More than two tiles of 16 columns go to the kernel of large tiles.
-// - Keys are split to one workgroup a CU (512, 768 or 1024 of them: slower, by their joins), in whole turns of the four
-//   waves.  A sequence of up to 12 blocks is not split: three blocks a wave cost less than the second launch.
-// - From 160 large tiles on, no split: the parts of many rows cost more than the CUs left idle (28 tiles of 1701 keys times
-//   8 heads, head_dim 64: 38 us (30) whole, 42 (36) split; 192 tiles of 2560 keys: 79 us (53), 81 (63)).
-// - Three key groups a workgroup where it has 24 blocks or more and the workgroups are less than two a CU (384 tiles of 64
-//   blocks: 129 us (84), one key group 158 (108)), else one (384 tiles of 8 blocks: 37 us (33), 31 (22); 768 of 64:
-//   229 us (152), 206 (140)).
+// Rows and keys over the workgroups; bf16 in parentheses where both types were timed (12 / 2 heads of 128 unless stated).
+// - Up to four tiles of 16 columns go to the kernel that reads the cache into registers, two of them a workgroup, more to
+//   the kernel of large tiles: 64 sequences of 4000 tokens with 5 fp32 rows (four tiles) 47 us, as a large tile 68; with 6
+//   rows (five) 81 and 70.
+// - Few rows: keys split to one workgroup a CU (512, 768 or 1024 of them: slower, by their joins), in whole turns of the
+//   four waves.  A sequence of up to 12 blocks is not split: three blocks a wave cost less than the second launch.
+// - Large tiles: keys split so that the workgroups come to one a CU at most, two blocks or more each (512 rows after 32000
+//   tokens of one sequence: 203 us (129); one a CU or a little more, which leaves some CUs two: 242 (158)).
+// - Several key groups a workgroup where each workgroup has a CU to itself and 12 blocks or more (28 / 4 heads of 64, 204
+//   tiles of 19 blocks: 30 us (24), one key group 34 (27)), or up to two a CU and 24 blocks (384 tiles of 64 blocks: 124 us
+//   (80), 155 (107); 264 of 22: 67 (50), 62 (45)); else one (384 tiles of 8 blocks: several 37 us (33), one 31 (22); 768 of
+//   64: 229 (152), 206 (140)).
 Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, int batch, int rows, int max_keys) {
+  constexpr int kCus = 256;
   const bool two = type == QWEN_TYPE_F32;
   const long long R = (long long)rows * (q_heads / c.kv_heads);
   const long long per_tile = two ? 8 : 16, tiles = (R + per_tile - 1) / per_tile;
   Kv8AttnPlan p{};
-  p.tiles = tiles > 2 ? 4 : (int)tiles;
-  p.tile_rows = p.tiles == 4 ? kKv8TileRows : (int)(p.tiles * per_tile);
+  p.large = tiles > 4;
+  p.tiles = tiles > 1 ? 2 : 1;
+  p.tile_rows = p.large ? kKv8TileRows : (int)(p.tiles * per_tile);
   p.groups = (int)((R + p.tile_rows - 1) / p.tile_rows);
   const long long blocks = (max_keys + kKv8Block - 1) / kKv8Block;
   const long long others = (long long)p.groups * c.kv_heads * batch;
-  long long per = (blocks * others + 255) / 256;
-  if (p.tiles == 4 && others >= 160) per = blocks;
-  if (per < 4) per = blocks <= 12 ? blocks : 4;
+  long long per;
+  if (p.large) {
+    const long long splits = others < kCus ? kCus / others : 1;
+    per = (blocks + splits - 1) / splits;
+    if (per < 2) per = 2;
+  } else {
+    per = (blocks * others + kCus - 1) / kCus;
+    if (per < 4) per = blocks <= 12 ? blocks : 4;
+    per = (per + 3) / 4 * 4;
+  }
   const long long least = (blocks + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (per < least) per = least;
-  per = (per + 3) / 4 * 4;
   p.per_split = (int)per;
   p.nsplit = (int)((blocks + per - 1) / per);
-  p.one_key_group = per < 24 || others * p.nsplit >= 512;
+  const long long workgroups = others * p.nsplit;
+  p.one_key_group = per < 12 || workgroups >= 2 * kCus || (per < 24 && workgroups > kCus);
   if (p.nsplit > 1)
     p.workspace = (size_t)batch * q_heads * rows * p.nsplit * (size_t)(c.head_dim + 2) * sizeof(float);
   return p;
