@@ -158,6 +158,17 @@ def test_full_vocabulary(torch):
           top_p=[0.95, 1.0, 0.5, 0.99, 0.9, 1.0] * 2, min_p=[0.0, 0.02] * 6)
 
 
+@pytest.mark.parametrize("vocab", [524288, 524289, 1300003])
+def test_longer_vocabularies(torch, vocab):
+    """More tokens than segments of one width hold, aligned rows and others: no cut, cuts with and without a list, ties."""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((5, vocab)) * 2.0
+    x[2] = np.round(x[2])
+    x[3] = rng.standard_normal(vocab) * 1e-5
+    x[3, 5] = 9.0
+    check(torch, x, rng.random(5), top_k=[0, 40, 0, 70000, 300000], top_p=[1.0, 0.9, 0.6, 0.9, 0.8], min_p=[0.0, 0.0, 0.0, 0.0, 1e-4])
+
+
 def test_draws_follow_the_distribution(torch):
     """Evenly spread uniforms hit every kept token in proportion, exactly (no tolerance: the draw is an inverse)."""
     x = np.log(np.array([1.0, 2.0, 4.0, 8.0, 1.0], np.float32))

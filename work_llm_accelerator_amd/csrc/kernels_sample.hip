@@ -4,11 +4,13 @@
 // ties by index, so a kept set is {key > T} and the first n of {key == T}; min-p is a test per token.  Weights are
 // 64-bit integers (fixed point), so sums are exact whatever the order of their atomics.
 //
-// Six launches, each over all rows: the row's maximum and minimum; a histogram (counts and weights) over 2048 equal
-// steps of the logit below the maximum; a list of the tokens of the steps in which top-k and top-p cut; the exact
-// (T, n) from that list; the kept weight of each segment of the row; the draw.  Rows are split over many blocks
-// except in the two launches that end in one number (the cut and the draw).  A row with a small k lists everything
-// down to the step of its cut: its weights are those of the list only, and the draw is made from it too.
+// Four launches, each over all rows: the row's maximum and minimum; a histogram (counts and weights) over 2048 equal
+// steps of the logit below the maximum (only where top-k or top-p is given); a list of the tokens of the steps in
+// which they cut, and of each segment of the row the weight of the tokens in steps that are kept whatever the cut; the
+// exact (T, n) from the list, and the draw: the listed tokens that are kept join their segments, the goal is found in
+// the segments' running sum and then among the tokens of one segment.  Rows are split over many blocks except in
+// the last launch.  A row with a small k lists everything down to the step of its cut: its weights are those of
+// the list only.
 #include <hip/hip_runtime.h>
 
 #include "kernels.hpp"
@@ -18,16 +20,17 @@ namespace qwen {
 
 namespace {
 
-constexpr int kThreads = 1024;
 constexpr int kBuckets = 2048;
 constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row)
 constexpr int kSmall = 2048;    // largest k whose row is decided by its list
-constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kThreads * 512 tokens)
+constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kMaxSegments * 512 tokens)
+constexpr int kMaxSegments = 1024;
 constexpr int kMaxChunks = 256;
-constexpr int kRed = kThreads / 64;  // words for the waves of a block (and two a wave of the chunks' maxima)
+constexpr int kRed = 16;  // words for the waves of a block (and two a wave of the chunks' maxima)
 constexpr uint32_t kUnlisted = 0xFFFFFFFFu;
 constexpr int kChunkThreads = 256;
 constexpr int kHistThreads = 512;
+constexpr int kCutThreads = 256;  // (512: one row 1 us more, 64 rows 0.5 less; 1024: 4 and 1.4 more)
 
 __device__ __forceinline__ float logit_at(const float* p, int i) { return p[i]; }
 __device__ __forceinline__ float logit_at(const uint16_t* p, int i) { return bits_f32((uint32_t)p[i] << 16); }
@@ -109,8 +112,6 @@ struct RowSpace {
   uint32_t listed;
   int k_step, p_low, p_high;  // the steps in the list (Needed)
   u64 k_before;
-  Cut cut;
-  int drawn;                  // the row's token is written
 };
 
 struct Sampler {
@@ -120,9 +121,9 @@ struct Sampler {
   int chunks, per_chunk;            // blocks that share a row: maxima,
   int hist_chunks, hist_per_chunk;  // histogram and list
   int segments, blocks_per_segment;  // of kSegment tokens
+  int segments_per_chunk;            // list
   RowSpace* space;
-  u64* seg_weight;     // [rows][segments]
-  uint32_t* seg_ties;  // [rows][segments]
+  u64* seg_weight;  // [rows][segments]
 };
 
 // 2^(t + bits) for t <= 0, 0 where t is below -110: Taylor's series over half a binade each way, degree 12 (its remainder
@@ -205,21 +206,43 @@ __device__ __forceinline__ const T* row_of(const SampleArgs& a, int row) {
   return static_cast<const T*>(a.logits) + row * a.row_stride;
 }
 
-// f(logit, index) over a block's chunk of `per` tokens of a row, eight loads in flight a thread (N of them).
-template <int N, class T, class F>
-__device__ __forceinline__ void over_chunk(const T* x, int vocab, int per, F&& f) {
-  constexpr int kAhead = 8;
-  const int end = min(vocab, ((int)blockIdx.x + 1) * per);
-  for (int i0 = blockIdx.x * per + threadIdx.x; i0 < end; i0 += kAhead * N) {
-    float v[kAhead];
+// The logits of 16 bytes.
+__device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
+  v[0] = bits_f32(q.x), v[1] = bits_f32(q.y), v[2] = bits_f32(q.z), v[3] = bits_f32(q.w);
+}
+__device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = logit_at(x, min(i0 + j * N, end - 1));
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i0 + j * N < end) f(v[j], i0 + j * N);
-  }
+  for (int i = 0; i < 4; ++i) v[2 * i] = bits_f32(w[i] << 16), v[2 * i + 1] = bits_f32(w[i] & 0xFFFF0000u);
 }
 
+// f(logit, index) over a block's chunk of `per` tokens of a row, four loads of 16 bytes in flight a thread (N of them);
+// the tokens before the first 16-byte boundary and behind the last one come alone.
+template <int N, class T, class F>
+__device__ __forceinline__ void over_chunk(const T* x, int vocab, int per, F&& f) {
+  constexpr int kAhead = 4, kVec = 16 / sizeof(T);
+  const int begin = blockIdx.x * per, end = min(vocab, begin + per), tid = threadIdx.x;
+  const int head = min(end - begin, (int)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16 / sizeof(T)));
+  const int first = begin + head, pieces = (end - first) / kVec, tail = first + pieces * kVec;
+  const uint4* at = reinterpret_cast<const uint4*>(x + first);
+  for (int p0 = tid; p0 < pieces; p0 += kAhead * N) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) q[j] = at[min(p0 + j * N, pieces - 1)];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (p0 + j * N >= pieces) break;
+      float v[kVec];
+      unpack(q[j], v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f(v[e], first + (p0 + j * N) * kVec + e);
+    }
+  }
+  if (tid < head) f(logit_at(x, begin + tid), begin + tid);
+  if (tail + tid < end) f(logit_at(x, tail + tid), tail + tid);
+}
+
+// Bound by the read: 64 rows of 151936 fp32 9.4 us, 4.1 TB/s (with 4-byte loads 10.6); one row 3.2 us, the launch.
 // grid = (chunks, rows).  Also clears the row's histogram.
 template <class T>
 __global__ void __launch_bounds__(kChunkThreads) sample_max_kernel(Sampler s) {
@@ -257,6 +280,7 @@ __device__ __forceinline__ bool wants_top_p(const Sampler& s, int row, float& p)
   return p < 1.0f;
 }
 
+// 64 rows of 151936, 8 of them with weights: 18 us; 10 without any weights: what they add is arithmetic in 64 bits.
 // grid = (chunks, rows).
 template <class T>
 __global__ void __launch_bounds__(kHistThreads) sample_hist_kernel(Sampler s) {
@@ -389,37 +413,23 @@ __device__ Needed needed_steps(const Held<N>& h, bool top_k, int k, bool top_p, 
   return n;
 }
 
-// Lists the needed steps' tokens; every block finds the steps for itself.  grid = (chunks, rows).
+// A lane's kLane adjacent tokens from `first` on (-inf behind the row): 16-byte loads where they are whole and aligned.
+constexpr int kLane = kSegment / 64;
 template <class T>
-__global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
-  __shared__ u64 red[kRed], pick[4];
-  __shared__ uint32_t pick_step, found, at;
-  __shared__ u64 keys[kList];
-  const int row = blockIdx.y, tid = threadIdx.x;
-  int k;
-  float p;
-  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
-  if (!top_k && !top_p) return;
-  RowSpace& w = s.space[row];
-  Held<kHistThreads> held(w);
-  const Row r(s, row, red);
-  if (r.greedy) return;
-  held.scan(red);
-  if (tid == 0) found = 0u;
-  const Needed need = needed_steps(held, top_k, k, top_p, p, pick, &pick_step);
-  if (blockIdx.x == 0 && tid == 0) {
-    w.k_step = need.k_step, w.p_low = need.low, w.p_high = need.high, w.k_before = need.k_before;
-    if (!need.listed) w.listed = kUnlisted;
+__device__ __forceinline__ void load_lane(const T* x, int first, int vocab, float (&v)[kLane]) {
+  constexpr int kVec = 16 / sizeof(T);
+  if (first + kLane <= vocab && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+#pragma unroll
+    for (int n = 0; n < kLane / kVec; ++n) {
+      float part[kVec];
+      unpack(reinterpret_cast<const uint4*>(x + first)[n], part);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[kVec * n + e] = part[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) v[j] = first + j < vocab ? logit_at(x, first + j) : -__builtin_inff();
   }
-  if (!need.listed) return;
-  const T* x = row_of<T>(s.a, row);
-  over_chunk<kHistThreads>(x, s.a.vocab, s.hist_per_chunk, [&](float v, int i) {
-    if (need.has(r.step(v))) keys[atomicAdd(&found, 1u)] = ((u64)order_key(v) << 32) | (u64)(uint32_t)i;
-  });
-  __syncthreads();
-  if (tid == 0 && found) at = atomicAdd(&w.listed, found);  // one a block: they are serialized over the row
-  __syncthreads();
-  for (int i = tid; i < (int)found; i += kHistThreads) w.list[at + i] = keys[i];
 }
 
 // The kept weight of a logit, without regard to ties.
@@ -432,41 +442,102 @@ __device__ __forceinline__ double least_weight(const Sampler& s, int row) {
   return q > 0.0f ? (double)fminf(q, 1.0f) * (double)(1ull << s.unit_bits) : 0.0;
 }
 
-// The cuts of one row, and its draw where the list holds all that is kept: grid = rows.
+// Lists the needed steps' tokens, and adds up the weight of those in steps that are kept whatever the cut: a wave per
+// segment, in turn.  Every block finds the steps for itself.  64 rows of 151936: 27.5 us, one row 10, of which finding
+// the steps takes 5.  grid = (chunks of segments, rows).
 template <class T>
-__global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
+__global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
+  __shared__ u64 red[kRed], pick[4];
+  __shared__ uint32_t pick_step, found, at;
+  __shared__ u64 keys[kList];
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  int k;
+  float p;
+  const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
+  RowSpace& w = s.space[row];
+  Held<kHistThreads> held(w);
+  const double least = least_weight(s, row);
+  const Row r(s, row, red);
+  if (r.greedy) return;
+  Needed need{-1, kBuckets, -1, 0, true};
+  int sure = kBuckets;  // tokens of the steps before it are kept
+  if (top_k || top_p) {
+    held.scan(red);
+    need = needed_steps(held, top_k, k, top_p, p, pick, &pick_step);
+    if (top_p || small_k(top_k, k))
+      sure = need.low;
+    else if (need.k_step >= 0)
+      sure = need.k_step;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    w.k_step = need.k_step, w.p_low = need.low, w.p_high = need.high, w.k_before = need.k_before;
+    if (!need.listed) w.listed = kUnlisted;
+  }
+  if (!need.listed) return;
+  if (tid == 0) found = 0u;
+  __syncthreads();
+  const T* x = row_of<T>(s.a, row);
+  const int last = min(s.segments, ((int)blockIdx.x + 1) * s.segments_per_chunk);
+  for (int seg = blockIdx.x * s.segments_per_chunk + (tid >> 6); seg < last; seg += kHistThreads / 64) {
+    u64 sum = 0;
+    for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
+      const int first = (seg * s.blocks_per_segment + blk) * kSegment + kLane * lane;
+      float v[kLane];
+      load_lane(x, first, s.a.vocab, v);
+#pragma unroll
+      for (int j = 0; j < kLane; ++j) {
+        if (first + j >= s.a.vocab) break;
+        const int b = r.step(v[j]);
+        if (need.has(b))
+          keys[atomicAdd(&found, 1u)] = ((u64)order_key(v[j]) << 32) | (u64)(uint32_t)(first + j);
+        else if (b < sure)
+          sum += kept_weight(r, v[j], least);
+      }
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s.seg_weight[(size_t)row * s.segments + seg] = sum;
+  }
+  __syncthreads();
+  if (tid == 0 && found) at = atomicAdd(&w.listed, found);  // one a block: they are serialized over the row
+  __syncthreads();
+  for (int i = tid; i < (int)found; i += kHistThreads) w.list[at + i] = keys[i];
+}
+
+// The cuts of one row, and its draw: a chain of reductions over one block, bound by their latency (64 rows 22.5 us, one row 15).
+// grid = rows.
+template <class T>
+__global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
   __shared__ u64 hist[kBuckets];
   __shared__ uint32_t count[kBuckets];
   __shared__ u64 list[kList], list_weight[kList];
+  __shared__ u64 seg_weight[kMaxSegments];
+  __shared__ uint32_t seg_ties[kMaxSegments];
   __shared__ u64 red[kRed], pick[4];
   __shared__ uint32_t pick_step, differ, sample_key;
-  const int row = blockIdx.x, tid = threadIdx.x, vocab = s.a.vocab;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, vocab = s.a.vocab;
   Cut cut{0u, 0u};  // everything: every key is above 0 (-inf has key 0x007FFFFF)
   int k;
   float p;
   const bool top_k = wants_top_k(s, row, k), top_p = wants_top_p(s, row, p);
   RowSpace& w = s.space[row];
-  if (!top_k && !top_p) {
-    if (tid == 0) w.cut = cut, w.drawn = 0;
-    return;
-  }
   const uint32_t listed = w.listed;
   Needed need{w.k_step, w.p_low, w.p_high, w.k_before, listed != kUnlisted};
   const bool small = small_k(top_k, k);
   const float uf = s.a.uniforms[row];
   const double least = least_weight(s, row);
-  Held<kChunkThreads> held(w);
+  Held<kCutThreads> held(w);
+  for (int i = tid; i < s.segments; i += kCutThreads) seg_weight[i] = s.seg_weight[(size_t)row * s.segments + i], seg_ties[i] = 0;
   if (need.listed)
-    for (int i = tid; i < (int)listed; i += kChunkThreads) list[i] = w.list[i];
+    for (int i = tid; i < (int)listed; i += kCutThreads) list[i] = w.list[i];
   const Row r(s, row, red);
   if (r.greedy) {
-    if (tid == 0) s.a.token_ids[row] = r.top_index, w.drawn = 1;
+    if (tid == 0) s.a.token_ids[row] = r.top_index;
     return;
   }
   const T* x = row_of<T>(s.a, row);
-  if (!small) held.scan(red);
+  if (top_p && !small) held.scan(red);
   if (top_p && need.listed)  // (each thread the entries that it has copied)
-    for (int i = tid; i < (int)listed; i += kChunkThreads) list_weight[i] = r.fixed(logit_of_key((uint32_t)(list[i] >> 32)));
+    for (int i = tid; i < (int)listed; i += kCutThreads) list_weight[i] = r.fixed(logit_of_key((uint32_t)(list[i] >> 32)));
 
   // Selects in falling order of 32-bit keys among candidates get(i, key), i < n, plus extra.ties more at extra.key, with
   // `above` in front of them: the key T at which a rank ends and the number of candidates at T within it.  The
@@ -480,12 +551,12 @@ __global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
     auto candidate = [&](int i, uint32_t& key) { return get(i, key) && (known == 32 || (key >> known) == prefix); };
     auto within = [&](u64 v) { return rank == kCount ? v < limit : rank == kBelow ? (double)v < goal : !((double)v > goal); };
     for (;;) {
-      for (int i = tid; i < kBuckets; i += kChunkThreads) hist[i] = 0, count[i] = 0;
+      for (int i = tid; i < kBuckets; i += kCutThreads) hist[i] = 0, count[i] = 0;
       if (tid == 0) differ = 0u, sample_key = 0u, pick_step = 0xFFFFFFFFu;
       __syncthreads();
       const bool extra_now = extra.ties && (known == 32 || (extra.key >> known) == prefix);
       uint32_t key, mine = 0, lo = 0xFFFFFFFFu;
-      for (int i = tid; i < n; i += kChunkThreads)
+      for (int i = tid; i < n; i += kCutThreads)
         if (candidate(i, key)) mine = max(mine, key), lo = min(lo, key);
       if (extra_now && tid == 0) mine = max(mine, extra.key), lo = min(lo, extra.key);
       if (mine) atomicMax(&sample_key, mine);
@@ -497,7 +568,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
       const uint32_t bits_off = differ;
       const int hb = bits_off ? 31 - __clz((int)bits_off) : -1, shift = max(0, hb - 10), bits = hb + 1 - shift;
       const uint32_t mask = bits ? (1u << bits) - 1u : 0u;
-      for (int i = tid; i < n; i += kChunkThreads) {
+      for (int i = tid; i < n; i += kCutThreads) {
         if (!candidate(i, key)) continue;
         const uint32_t bucket = (key >> shift) & mask;
         atomicAdd(&count[bucket], 1u);
@@ -527,12 +598,12 @@ __global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
         return c;
       }
       // this thread's adjacent buckets, the largest first; the smallest non-empty one that starts within the rank
-      constexpr int kPer = kBuckets / kChunkThreads;
+      constexpr int kPer = kBuckets / kCutThreads;
       const int hi = kBuckets - 1 - kPer * tid;
       u64 b[kPer], sum = 0, total, my_before = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) b[i] = rank == kCount ? count[hi - i] : hist[hi - i], sum += b[i];
-      u64 run = above + block_scan<kChunkThreads>(sum, red, total);
+      u64 run = above + block_scan<kCutThreads>(sum, red, total);
       uint32_t my = 0xFFFFFFFFu;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -576,12 +647,12 @@ __global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
   auto weight_of = [&](int step) {
     u64 part = 0, total;
     const int n = need.listed ? (int)listed : vocab;
-    for (int i = tid; i < n; i += kChunkThreads) {
+    for (int i = tid; i < n; i += kCutThreads) {
       const uint32_t key = need.listed ? list_key(i) : order_key(logit_at(x, i));
       if (key > cut.key && (step < 0 || r.step(logit_of_key(key)) == step)) part += key_weight(i, key);
     }
     if (tid == 0 && cut.ties) part += cut.ties * r.fixed(logit_of_key(cut.key));
-    block_scan<kChunkThreads>(part, red, total);
+    block_scan<kCutThreads>(part, red, total);
     return total;
   };
 
@@ -599,152 +670,120 @@ __global__ void __launch_bounds__(kChunkThreads) sample_cut_kernel(Sampler s) {
       total += last_weight;
     }
     const double goal = (double)p * (double)total;
-    if (!(goal > 0.0)) {
-      cut = Cut{r.top_key, 1u};
-    } else if (small || !need.listed) {
+    if (!(goal > 0.0)) {  // (p <= 0: the first token alone)
+      if (tid == 0) s.a.token_ids[row] = r.top_index;
+      return;
+    }
+    if (small || !need.listed) {
       cut = top_p_cut(-1, 0, goal, cut);
     } else {
       const auto f = held.find(true, 0, goal, last, last_weight, pick, &pick_step);
       cut = top_p_cut(f.step, f.before, goal, f.step == last ? cut : Cut{0u, 0u});
     }
   }
-  if (!small || !need.listed) {
-    if (tid == 0) w.cut = cut, w.drawn = 0;
-    return;
-  }
-  // The draw from the list: the last index (in rising order: the falling one of ~index) of the ties that are kept, then the
-  // index at which the running weight passes the goal
-  const u64 tie = cut.ties ? kept_weight(r, logit_of_key(cut.key), least) : 0ull;
-  const Cut end = cut.ties ? select((int)listed, [&](int i, uint32_t& key) { key = ~(uint32_t)list[i]; return list_key(i) == cut.key; },
-                                    key_weight, 0, kCount, cut.ties, 0.0, Cut{0u, 0u}, Cut{0u, 0u})
-                           : Cut{0xFFFFFFFFu, 0u};
-  u64 sum = 0, total;
-  for (int i = tid; i < (int)listed; i += kChunkThreads) {
-    const uint32_t key = list_key(i);
-    list_weight[i] = key > cut.key ? kept_weight(r, logit_of_key(key), least)
-                                   : key == cut.key && ~(uint32_t)list[i] >= end.key ? tie : 0ull;
-    sum += list_weight[i];
-  }
-  block_scan<kChunkThreads>(sum, red, total);
-  const double goal = (uf > 0.0f ? (double)fminf(uf, 1.0f) : 0.0) * (double)total;
-  const Cut token = select((int)listed, [&](int i, uint32_t& key) { key = ~(uint32_t)list[i]; return list_weight[i] != 0; },
-                           key_weight, 0, kUpTo, 0, goal, Cut{0u, 0u}, Cut{~(uint32_t)r.top_index, 0u});
-  if (tid == 0) s.a.token_ids[row] = (int)~token.key, w.drawn = 1;
-}
 
-// Kept weight above the cut, and number of tokens at it, of each segment: a wave per segment, in turn.
-// grid = (blocks, rows).
-template <class T>
-__global__ void __launch_bounds__(kChunkThreads) sample_segment_kernel(Sampler s) {
-  __shared__ u64 red[kRed];
-  const int row = blockIdx.y, lane = threadIdx.x & 63;
-  const T* x = row_of<T>(s.a, row);
-  if (s.space[row].drawn) return;
-  const Cut cut = s.space[row].cut;
-  const double least = least_weight(s, row);
-  const Row r(s, row, red);
-  if (r.greedy) return;
-  for (int seg = blockIdx.x * (kChunkThreads / 64) + (threadIdx.x >> 6); seg < s.segments; seg += gridDim.x * (kChunkThreads / 64)) {
-    u64 w = 0;
-    uint32_t n = 0;
-    for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
-      const int i0 = (seg * s.blocks_per_segment + blk) * kSegment + lane;
-      float v[kSegment / 64];
-#pragma unroll
-      for (int j = 0; j < kSegment / 64; ++j) v[j] = i0 + 64 * j < s.a.vocab ? logit_at(x, i0 + 64 * j) : -__builtin_inff();
-#pragma unroll
-      for (int j = 0; j < kSegment / 64; ++j) {
-        const uint32_t key = order_key(v[j]);
-        if (key > cut.key) w += kept_weight(r, v[j], least);
-        if (key == cut.key && i0 + 64 * j < s.a.vocab) ++n;
+  // Each segment's kept weight above the cut, and its tokens at it
+  if (need.listed) {
+    for (int i = tid; i < (int)listed; i += kCutThreads) {
+      const uint32_t key = list_key(i);
+      const int seg = (int)(uint32_t)list[i] / (kSegment * s.blocks_per_segment);
+      if (key > cut.key) {
+        const u64 n = kept_weight(r, logit_of_key(key), least);
+        if (n) atomicAdd(&seg_weight[seg], n);
+      } else if (key == cut.key) {
+        atomicAdd(&seg_ties[seg], 1u);
       }
     }
-    w = wave_sum(w);
-    n = wave_sum(n);
-    if (lane == 0) {
-      s.seg_weight[(size_t)row * s.segments + seg] = w;
-      s.seg_ties[(size_t)row * s.segments + seg] = n;
+  } else {
+    for (int seg = tid >> 6; seg < s.segments; seg += kCutThreads / 64) {
+      u64 sum = 0;
+      uint32_t n = 0;
+      for (int i = seg * s.blocks_per_segment * kSegment + lane; i < min(vocab, (seg + 1) * s.blocks_per_segment * kSegment); i += 64) {
+        const float v = logit_at(x, i);
+        const uint32_t key = order_key(v);
+        if (key > cut.key) sum += kept_weight(r, v, least);
+        if (key == cut.key) ++n;
+      }
+      sum = wave_sum(sum);
+      n = wave_sum(n);
+      if (lane == 0) seg_weight[seg] = sum, seg_ties[seg] = n;
     }
   }
-}
-
-// The draw: the segment that holds the goal, then the token in it.  One segment a thread; grid = rows.
-template <class T>
-__global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
-  __shared__ u64 red[kRed];
-  __shared__ u64 pick_above;
-  __shared__ uint32_t pick_segment, pick_seen;
-  const int row = blockIdx.x, tid = threadIdx.x;
-  if (s.space[row].drawn) return;
-  // everything that the row's weights do not decide, before the first wait
-  const bool live = tid < s.segments;
-  const u64 my_weight = live ? s.seg_weight[(size_t)row * s.segments + tid] : 0ull;
-  const u64 my_ties = live ? s.seg_ties[(size_t)row * s.segments + tid] : 0ull;
-  const Cut cut = s.space[row].cut;
-  const double least = least_weight(s, row);
-  const float uf = s.a.uniforms[row];
-  const Row r(s, row, red);
-  if (r.greedy) {
-    if (tid == 0) s.a.token_ids[row] = r.top_index;
-    return;
-  }
+  if (tid == 0) pick_step = 0u;
+  __syncthreads();
+  // The last segment with kept weight that starts at or below the goal; a thread has kPer adjacent ones
+  constexpr int kPer = kMaxSegments / kCutThreads;
   const u64 tie = cut.ties ? kept_weight(r, logit_of_key(cut.key), least) : 0ull;
-  u64 none, total;
-  const u64 seen = block_scan<kThreads>(my_ties, red, none);
-  const u64 kept = seen >= cut.ties ? 0ull : min(my_ties, (u64)cut.ties - seen);
-  const u64 weight = my_weight + kept * tie;
-  const u64 before = block_scan<kThreads>(weight, red, total);
+  u64 weight[kPer], sum = 0, none, total, my_above = 0, my_seen = 0;
+  uint32_t ties[kPer], all_ties = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool live = kPer * tid + i < s.segments;
+    ties[i] = live ? seg_ties[kPer * tid + i] : 0u, weight[i] = live ? seg_weight[kPer * tid + i] : 0ull;
+    all_ties += ties[i];
+  }
+  u64 seen = block_scan<kCutThreads>(all_ties, red, none);
+  const u64 seen_first = seen;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    weight[i] += (seen >= cut.ties ? 0ull : min((u64)ties[i], (u64)cut.ties - seen)) * tie;
+    seen += ties[i];
+    sum += weight[i];
+  }
+  u64 run = block_scan<kCutThreads>(sum, red, total);
   const double goal = (uf > 0.0f ? (double)fminf(uf, 1.0f) : 0.0) * (double)total;
-  // the last segment with kept weight that starts at or below the goal
-  const bool within = weight && !((double)before > goal);
-  if (tid == 0) pick_segment = 0u;
+  int mine = -1;
+  seen = seen_first;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (weight[i] && !((double)run > goal)) mine = kPer * tid + i, my_above = run, my_seen = seen;
+    run += weight[i];
+    seen += ties[i];
+  }
+  if (mine >= 0) atomicMax(&pick_step, (uint32_t)mine);
   __syncthreads();
-  if (within) atomicMax(&pick_segment, (uint32_t)tid);
-  __syncthreads();
-  if (tid == (int)pick_segment) pick_above = before, pick_seen = (uint32_t)seen;
+  const int segment = (int)pick_step;
+  if (mine == segment) pick[0] = my_above, pick[1] = my_seen;
   __syncthreads();
   if (tid >= 64) return;
-  // one wave: each lane eight adjacent tokens
-  constexpr int kLane = kSegment / 64;
-  const T* x = row_of<T>(s.a, row);
-  u64 above = pick_above;
-  uint32_t rank0 = pick_seen;
+  // The token: one wave, each lane eight adjacent tokens
+  u64 above = pick[0];
+  uint32_t rank0 = (uint32_t)pick[1];
   int token = 0;
   for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
-    const int first = ((int)pick_segment * s.blocks_per_segment + blk) * kSegment + kLane * tid;
+    const int first = (segment * s.blocks_per_segment + blk) * kSegment + kLane * tid;
     float v[kLane];
+    load_lane(x, first, vocab, v);
+    uint32_t at_cut = 0;
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) v[j] = first + j < s.a.vocab ? logit_at(x, first + j) : -__builtin_inff();
-    uint32_t held = 0;
-#pragma unroll
-    for (int j = 0; j < kLane; ++j) held += first + j < s.a.vocab && order_key(v[j]) == cut.key ? 1u : 0u;
-    uint32_t rank = wave_scan(held);
+    for (int j = 0; j < kLane; ++j) at_cut += first + j < vocab && order_key(v[j]) == cut.key ? 1u : 0u;
+    uint32_t rank = wave_scan(at_cut);
     const uint32_t rank_next = rank0 + last_lane(rank);
-    rank += rank0 - held;
-    u64 here[kLane], sum = 0;
+    rank += rank0 - at_cut;
+    u64 here[kLane], part = 0;
 #pragma unroll
     for (int j = 0; j < kLane; ++j) {
       const uint32_t key = order_key(v[j]);
       here[j] = key > cut.key ? kept_weight(r, v[j], least) : 0ull;
-      if (first + j < s.a.vocab && key == cut.key && rank++ < cut.ties) here[j] = tie;
-      sum += here[j];
+      if (first + j < vocab && key == cut.key && rank++ < cut.ties) here[j] = tie;
+      part += here[j];
     }
-    u64 run = wave_scan(sum);
-    const u64 above_next = above + last_lane(run);
-    run += above - sum;
+    u64 upto = wave_scan(part);
+    const u64 above_next = above + last_lane(upto);
+    upto += above - part;
     int past = -1, some = -1;  // the lane's first token beyond the goal, and its last one with weight
 #pragma unroll
     for (int j = 0; j < kLane; ++j) {
-      run += here[j];
+      upto += here[j];
       if (here[j]) {
         some = j;
-        if (past < 0 && (double)run > goal) past = j;
+        if (past < 0 && (double)upto > goal) past = j;
       }
     }
     const u64 beyond = __ballot(past >= 0), any = __ballot(some >= 0);
     if (any) {
-      const int lane = beyond ? __ffsll(beyond) - 1 : 63 - __clzll(any);
-      token = __shfl(first + (beyond ? past : some), lane, 64);
+      const int from = beyond ? __ffsll(beyond) - 1 : 63 - __clzll(any);
+      token = __shfl(first + (beyond ? past : some), from, 64);
     }
     if (beyond) break;
     above = above_next;
@@ -756,27 +795,24 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(Sampler s) {
 template <class T>
 void run_sample(const Sampler& s, hipStream_t st) {
   const int rows = s.a.rows;
-  const int segment_blocks = (s.segments + 3) / 4;
   hipLaunchKernelGGL(sample_max_kernel<T>, dim3(s.chunks, rows), dim3(kChunkThreads), 0, st, s);
-  if (s.a.top_k || s.a.top_p) {
+  if (s.a.top_k || s.a.top_p)
     hipLaunchKernelGGL(sample_hist_kernel<T>, dim3(s.hist_chunks, rows), dim3(kHistThreads), 0, st, s);
-    hipLaunchKernelGGL(sample_list_kernel<T>, dim3(s.hist_chunks, rows), dim3(kHistThreads), 0, st, s);
-  }
-  hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(rows), dim3(kChunkThreads), 0, st, s);
-  hipLaunchKernelGGL(sample_segment_kernel<T>, dim3(segment_blocks, rows), dim3(kChunkThreads), 0, st, s);
-  hipLaunchKernelGGL(sample_draw_kernel<T>, dim3(rows), dim3(kThreads), 0, st, s);
+  const int list_chunks = (s.segments + s.segments_per_chunk - 1) / s.segments_per_chunk;
+  hipLaunchKernelGGL(sample_list_kernel<T>, dim3(list_chunks, rows), dim3(kHistThreads), 0, st, s);
+  hipLaunchKernelGGL(sample_cut_kernel<T>, dim3(rows), dim3(kCutThreads), 0, st, s);
 }
 
 }  // namespace
 
-static int blocks_per_segment(int vocab) { return (vocab + kThreads * kSegment - 1) / (kThreads * kSegment); }
+static int blocks_per_segment(int vocab) { return (vocab + kMaxSegments * kSegment - 1) / (kMaxSegments * kSegment); }
 static int segments_of(int vocab) {
   const int tokens = blocks_per_segment(vocab) * kSegment;
   return (vocab + tokens - 1) / tokens;
 }
 
 size_t sample_workspace_bytes(int rows, int vocab) {
-  return (size_t)rows * (sizeof(RowSpace) + segments_of(vocab) * (sizeof(u64) + sizeof(uint32_t)));
+  return (size_t)rows * (sizeof(RowSpace) + segments_of(vocab) * sizeof(u64));
 }
 
 void launch_sample(const SampleArgs& a, void* workspace, hipStream_t st) {
@@ -795,14 +831,16 @@ void launch_sample(const SampleArgs& a, void* workspace, hipStream_t st) {
     chunks = (a.vocab + per - 1) / per;
   };
   split(1024, 1024, kChunkThreads, s.chunks, s.per_chunk);  // about four a CU over all rows, of 1024 tokens at least
-  // histogram and list: two of 512 threads a CU (64 rows of 151936: 22 + 19 us; 256 x 1024 threads 22 + 18 but one row
-  // 7 + 12 instead of 6 + 9 us; 1024 blocks of 256 threads 23 + 19 and 8 + 9; 512 of 1024 26 + 29)
+  // histogram: two of 512 threads a CU (64 rows of 151936: 18 us, and so with four or eight; one of 1024 threads the same, but
+  // one row 7 us instead of 6; four of 256 threads 1 and 2 us more; two of 1024 4 more)
   split(512, 4 * kHistThreads, kHistThreads, s.hist_chunks, s.hist_per_chunk);
   s.segments = segments_of(a.vocab);
   s.blocks_per_segment = blocks_per_segment(a.vocab);
+  // list: four blocks a CU (64 rows of 151936: 27.5 us; with two or eight 30, with one 33), a segment a wave at least
+  s.segments_per_chunk = (int)(((long long)s.segments * a.rows + 1023) / 1024);
+  if (s.segments_per_chunk < kHistThreads / 64) s.segments_per_chunk = kHistThreads / 64;
   s.space = static_cast<RowSpace*>(workspace);
   s.seg_weight = reinterpret_cast<u64*>(s.space + a.rows);
-  s.seg_ties = reinterpret_cast<uint32_t*>(s.seg_weight + (size_t)a.rows * s.segments);
   if (a.type == QWEN_TYPE_F32)
     run_sample<float>(s, st);
   else
