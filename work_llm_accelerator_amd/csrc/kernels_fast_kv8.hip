@@ -33,8 +33,8 @@ __device__ __forceinline__ uint32_t regrade(uint32_t w, float ratio) {
 // into registers, their largest magnitude gives the scale (a maximum of bit patterns: non-finite values come
 // out on top), and the codes are written once; V goes through LDS to turn 4 x 4 bytes.  The earlier rows of a
 // part-filled block are read only where the scale grows.  Bound by the stream of new rows: 8 x 2048 tokens (bf16, 2 heads
-// of 128) 8.4 us for 50 MB, out of the caches; single tokens by the launch and two round trips to memory: 4.8 us for one
-// sequence, 5.6 for 64.
+// of 128) 8.5 us for 25 MB, of which the launch takes 3; single tokens (fp32) by the launch and two round trips to memory:
+// 4.7 us for one sequence, 5.5 for 64.
 // grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
 template <class T, int D>
 __global__ void __launch_bounds__(256) kv8_store_kernel(qwen_kv8_cache c, qwen_kv8_rows kin, qwen_kv8_rows vin, int rows,
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) fill_i32_kernel(int* __restrict__ p, int 
 
 // ---- load -----------------------------------------------------------------------------------
 // The inverse, one block of 256 threads per (cache block, head, K or V, sequence); bound by the rows written: 4 x 32768
-// tokens (bf16, 2 heads of 128) 72 us for 336 MB, 4.7 TB/s where a copy reaches 5.2; with 8-byte stores 80 us, with
+// tokens (fp32, 2 heads of 128) 72 us for 336 MB, 4.7 TB/s where a copy reaches 5.2; with 8-byte stores 80 us, with
 // nontemporal ones 76 or 116 from run to run.
 // grid = (blocks that `rows` tokens can touch, 2 * kv_heads, batch).
 template <class T, int D>

@@ -13,6 +13,11 @@
 // groups of a workgroup (KG) take the blocks in turn, kept a part of a turn apart by barriers, and are joined at the
 // end.  One such prompt: 83 us, with KG = 1 96 to 108 (also as two splits, or as tiles of 64 rows with two key groups
 // of two waves: 98).
+//
+// Counters at four prompts: vector instructions issue in 54 % of the SIMDs' cycles, the matrix cores are busy in 35 %, LDS
+// instructions issue in 10 %: the two waves of a SIMD hide little of each other.  One wave that interleaves the scores of
+// its next block with its probabilities, and its products with the conversion (two buffers a tile, one barrier a block):
+// 272 us instead of 253.
 // fp32 rows enter as hi and lo fp16 terms in two products each, as their probabilities do.
 #include "kv8_device.hpp"
 
