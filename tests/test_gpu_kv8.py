@@ -303,6 +303,22 @@ def test_attend_large_tiles(torch, dtype, sequences, blocks, dim):
     assert (np.abs(got - want) <= tol)[~np.isnan(want)].all()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sequences,blocks,rows", [(2, 6, 3), (2, 6, 40), (80, 25, 17)])
+def test_attend_blocks_of_zeros(torch, dtype, sequences, blocks, rows):
+    """Blocks whose values are all zero, stored (the least scale) or never stored (a scale of 0), first, last and between
+    others: they weigh in the sum of the probabilities like any other."""
+    cache = filled(torch, sequences, blocks, 2, 64, 40 + rows)
+    for b in range(sequences):
+        for j in range(b % 4, blocks, 4 if b % 3 else 1 + b % 5):
+            cache.v[0, b, j] = 0
+            cache.v_scale[0, b, j] = 0.0 if b % 2 else 2.0 ** -126
+    cache.k[0, 1, 1], cache.k_scale[0, 1, 1] = 0, 2.0 ** -126
+    cache.k[0, 1, 2], cache.k_scale[0, 1, 2] = 0, 0.0
+    q, _ = rows_of(torch, np.random.default_rng(rows), (sequences, rows, 4, 64), dtype, 0.0)
+    check_attend(torch, cache, q, [64 * blocks - rows - 11 * (b % 5) for b in range(sequences)], 64 * blocks)
+
+
 def test_attend_non_finite_queries(torch):
     cache = filled(torch, 1, 2, 1, 64, 14)
     q = torch.ones(1, 4, 1, 64, device="cuda")

@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(K
   // ready for them; then the probabilities of each half of its tokens into p.
   float f = 0.0f, base = 0.0f, sum = 0.0f;
   int shift = 0;
+  bool drop = false;
   auto mask = [&](int key0) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -278,17 +279,22 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(K
     // the block's V scale is folded into the probabilities where it is a little below the accumulator's unit
     shift = unit - sv;
     base = m - kProbBits + (float)shift;
+    drop = false;
     const bool usual = most <= m + kProbLag && m > -__builtin_inff() && (uint32_t)shift <= (uint32_t)kTileFold;
     if (__all(usual)) return;
     const bool first = m == -__builtin_inff(), up = most > m + kProbLag || (first && most > m);
     const float mn = up ? most : m;
     const float alpha = up ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
-    // else the unit changes to it, unless none of its probabilities is large enough to be more than 0
+    // else the unit changes to it, unless none of its probabilities is large enough to be more than 0, or its values are
+    // below 2^-80 of what the accumulators may hold (a block of zeros: its scale is the least one, or 0): those
+    // count in the sum alone
     const bool touched = most > mn - (kProbBits + 25.0f);
-    const bool change = touched && (first || ((uint32_t)shift > (uint32_t)kTileFold && shift <= 80));
-    const float grow = __builtin_amdgcn_ldexpf(alpha, change && !first ? shift : 0);
+    const float lead = (float)shift + (up && !first ? m - mn : 0.0f);
+    const bool change = touched && (first || ((uint32_t)shift > (uint32_t)kTileFold && lead <= 80.0f));
+    const float grow = change && !first ? __builtin_amdgcn_exp2f(lead) : alpha;
+    drop = touched && !change && shift > kTileFold;
     unit = change ? sv : unit;
-    shift = change ? 0 : shift < 0 ? 400 : shift;
+    shift = change || drop ? 0 : shift < 0 ? 400 : shift;
     base = mn == -__builtin_inff() ? 0.0f : mn - kProbBits + (float)shift;
     m = mn;
     l *= alpha;
@@ -344,6 +350,11 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(K
       if constexpr (KG > 2) tick();
       probabilities(std::integral_constant<int, 1>{});
       l += __builtin_amdgcn_ldexpf(sum, shift);
+      if (__any(drop))
+#pragma unroll
+        for (int b2 = 0; b2 < kLimbs; ++b2)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) p[b2][u] = drop ? half8{} : p[b2][u];
       write_v();
       write_k();
       sk = a.c.k_scale[place(it + 1)];
