@@ -319,6 +319,32 @@ def test_attend_blocks_of_zeros(torch, dtype, sequences, blocks, rows):
     check_attend(torch, cache, q, [64 * blocks - rows - 11 * (b % 5) for b in range(sequences)], 64 * blocks)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,sequences,blocks", [(40, 1, 20), (17, 80, 25)])
+def test_attend_large_tiles_peaked_and_flat(torch, dtype, rows, sequences, blocks):
+    """Tiles of many rows: one token takes all, all tokens equal, scales of the attention of zero and below, maxima that
+    rise from block to block while the V scales fall and the other way round."""
+    cache = filled(torch, sequences, blocks, 2, 64, 7 + rows)
+    q, _ = rows_of(torch, np.random.default_rng(rows), (sequences, rows, 4, 64), dtype, 0.0)
+    pos = [64 * blocks - rows - 3 * (b % 9) for b in range(sequences)]
+    few = slice(0, min(3, sequences))
+
+    def check(x, scale):
+        part = type(cache)(*(t[:, few].contiguous() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+        want, slack, floor, reach = Cache.of(part).attend(x[few].float().cpu().numpy(), pos[few], scale)
+        got = cache.attend(0, x, ints(torch, pos), 64 * blocks, scale=scale)[few].float().cpu().numpy()
+        tol = tolerance("f32" if dtype == "float32" else "bf16", 64, slack, floor, reach, want)
+        assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) - tol)
+
+    for x, scale in ((q * 300, 0.125), (q * 0, 0.125), (q, 0.0), (q, -0.3)):
+        check(x, scale)
+    step = torch.arange(blocks, dtype=torch.float32, device="cuda")
+    for sign in (1, -1):
+        cache.k_scale[0] = torch.exp2(-9 + step * (6 / blocks))[:, None].log2().round().exp2()
+        cache.v_scale[0] = torch.exp2(sign * 4 * (step - blocks // 2))[:, None]
+        check(q * 8, 0.125)
+
+
 def test_attend_non_finite_queries(torch):
     cache = filled(torch, 1, 2, 1, 64, 14)
     q = torch.ones(1, 4, 1, 64, device="cuda")
@@ -345,6 +371,32 @@ def test_attend_strided_and_in_place(torch, dtype):
     assert torch.equal(flat, before)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sequences,blocks,rows", [(4, 20, 40), (80, 25, 17), (3, 5, 300)])
+def test_attend_large_tiles_in_place_and_captured(torch, dtype, sequences, blocks, rows):
+    """Results over the queries themselves, with and without key splits (also where one split holds all of a short
+    sequence), in a captured call that is replayed at other lengths."""
+    cache = filled(torch, sequences, blocks, 2, 64, 3 + rows)
+    rng = np.random.default_rng(rows)
+    source, _ = rows_of(torch, rng, (sequences, rows, 6, 64), dtype, 0.0)
+    q, pos = source.clone(), ints(torch, [0] * sequences)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attend(0, q, pos, 64 * blocks, out=q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        cache.attend(0, q, pos, 64 * blocks, out=q)
+    for turn in range(3):
+        pos.copy_(ints(torch, rng.integers(-1, 64 * blocks - rows + 1, sequences).tolist()))
+        q.copy_(source)
+        want = cache.attend(0, source, pos, 64 * blocks)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q, want)
+
+
 def test_python_refusals(torch):
     from work_llm_accelerator_amd.kv8 import Kv8Cache
 
@@ -365,6 +417,11 @@ def test_python_refusals(torch):
         cache.attend(0, x, pos, 129)
     with pytest.raises(ValueError):
         cache.attend(0, x, pos, 64, out=x.bfloat16())
+    for n in (0, -1, 2 ** 32 + 64):  # (as a C int the last one is 64)
+        with pytest.raises(ValueError):
+            cache.attend(0, x, pos, n)
+    with pytest.raises(ValueError):
+        cache.store(0, x[:, :1].expand(2, 2 ** 32 + 1, 2, 128), x[:, :1].expand(2, 2 ** 32 + 1, 2, 128), pos)
     with pytest.raises(ValueError):
         cache.load(0, pos)
     with pytest.raises(ValueError):

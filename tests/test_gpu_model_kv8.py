@@ -276,6 +276,8 @@ def test_refusals(torch, model):
                  lambda: model.decode_kv8(x, pos, 64, Kv8Cache.allocate(2, 2, 64, 4, 64)),
                  lambda: model.prefill_kv8(x.view(1, 2, HIDDEN), cache, past=63),
                  lambda: model.prefill_kv8(x.view(1, 2, HIDDEN), cache, past=-1),
+                 lambda: model.prefill_kv8(x.view(1, 2, HIDDEN), cache, past=2 ** 32),
+                 lambda: model.decode_kv8(x, pos, 2 ** 32 + 64, cache),
                  lambda: model.prefill_kv8(torch.zeros(1, 0, HIDDEN, device="cuda"), cache)):
         with pytest.raises((RuntimeError, ValueError)):
             call()

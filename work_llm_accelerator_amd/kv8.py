@@ -23,6 +23,7 @@ BLOCK = 64  # tokens that share a scale
 TYPE_F32 = 0
 TYPE_BF16 = 1
 ZERO_OUTSIDE = 0x1
+MAX_COUNT = 1 << 24
 
 
 def _check(lib, status: int, what: str) -> None:
@@ -118,6 +119,8 @@ class Kv8Cache:
         strides = t.stride()
         if t.shape != shape:
             raise ValueError(f"{what} must be {shape}, not {tuple(t.shape)}")
+        if shape[0] > MAX_COUNT or shape[1] > MAX_COUNT or shape[2] > MAX_COUNT:  # (ctypes would cut them to 32 bits)
+            raise ValueError(f"{what} has a dimension above {MAX_COUNT}")
         if t.device != self.k.device:
             raise ValueError(f"{what} must be on {self.k.device}, not {t.device}")
         if strides[3] != 1:
@@ -187,17 +190,20 @@ class Kv8Cache:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if out.dtype != q.dtype:
             raise ValueError("q and out must have one type")
+        max_keys = int(max_keys)
+        if not 0 < max_keys <= self.positions:
+            raise ValueError(f"max_keys must be 1 .. {self.positions}, not {max_keys}")
         shape = (batch, rows, heads, self.head_dim)
         qs, os = self._rows(q, shape, "q"), self._rows(out, shape, "out")
         pos, c, lib, kind = self._positions(positions, batch), self.layer_struct(layer), abi.load(), _type_of(q)
         need = ctypes.c_uint64(0)
         with _on(self.k.device):
-            _check(lib, lib.qwen_hip_kv8_attention_workspace(ctypes.byref(c), kind, heads, batch, rows, int(max_keys),
+            _check(lib, lib.qwen_hip_kv8_attention_workspace(ctypes.byref(c), kind, heads, batch, rows, max_keys,
                                                              ctypes.byref(need)), "qwen_hip_kv8_attention_workspace")
             # the stream's own allocation: reused by later work of this stream only, private to a graph being captured
             ws = torch.empty(need.value, dtype=torch.uint8, device=self.k.device) if need.value else None
             st = lib.qwen_hip_kv8_attention(ctypes.byref(c), kind, ctypes.byref(qs), ctypes.byref(os), heads, batch, rows,
-                                            pos, int(max_keys), 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
+                                            pos, max_keys, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
                                             ws.data_ptr() if ws is not None else None, need.value,
                                             _raw_stream(self.k.device.index))
         _check(lib, st, "qwen_hip_kv8_attention")

@@ -174,6 +174,8 @@ class DeviceModel:
         GPU (negative: inactive); flags 0 or FLAG_NO_BF16_ROUND; `layers` as in _range."""
         if order:
             self._enter()
+        if not 0 < max_keys <= cache.positions:
+            raise ValueError(f"max_keys must be 1 .. {cache.positions}, not {max_keys}")
         first, count, c = self._range_kv8(cache, layers)
         st = self.lib.qwen_hip_model_decode_kv8(self.handle, flags, first, count, hidden.shape[0], _ptr(hidden),
                                                 _ptr(positions), int(max_keys), ctypes.byref(c))
@@ -184,6 +186,8 @@ class DeviceModel:
         are stored as codes (tokens 0..past-1 are there already); flags and `layers` as in decode_kv8."""
         if order:
             self._enter()
+        if not 0 <= past <= cache.positions - hidden.shape[1]:
+            raise ValueError(f"past {past} and {hidden.shape[1]} tokens do not fit {cache.positions} positions")
         first, count, c = self._range_kv8(cache, layers)
         st = self.lib.qwen_hip_model_prefill_kv8(self.handle, flags, first, count, hidden.shape[0], hidden.shape[1],
                                                  int(past), _ptr(hidden), ctypes.byref(c))

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import abi
-from .kv8 import _check, _on, _raw_stream, _type_of
+from .kv8 import MAX_COUNT, _check, _on, _raw_stream, _type_of
 
 
 def row_params(rows: int, device, uniforms, temperature, top_k, top_p, min_p, token_ids) -> list:
@@ -39,6 +39,8 @@ def sample_logits(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
+    if rows > MAX_COUNT or vocab > MAX_COUNT:
+        raise ValueError(f"logits must be at most {MAX_COUNT} each way")
     if token_ids is None:
         token_ids = torch.empty(rows, dtype=torch.int32, device=logits.device)
     kind, lib = _type_of(logits), abi.load()
