@@ -21,7 +21,8 @@ namespace qwen {
 namespace {
 
 constexpr int kBuckets = 2048;
-constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row)
+constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row; 151936 normal
+                                // logits have up to 270 in a step)
 constexpr int kSmall = 2048;    // largest k whose row is decided by its list
 constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kMaxSegments * 512 tokens)
 constexpr int kMaxSegments = 1024;
@@ -504,6 +505,8 @@ __global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
 }
 
 // The cuts of one row, and its draw: a chain of reductions over one block, bound by their latency (64 rows 22.5 us, one row 15).
+// A row with more tokens in the cuts' steps than the list holds (nearly equal logits) is gone through whole here: 0.3 to
+// 0.9 ms for 151936 tokens, most of it atomics at the same address.
 // grid = rows.
 template <class T>
 __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
@@ -539,25 +542,42 @@ __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
   if (top_p && need.listed)  // (each thread the entries that it has copied)
     for (int i = tid; i < (int)listed; i += kCutThreads) list_weight[i] = r.fixed(logit_of_key((uint32_t)(list[i] >> 32)));
 
-  // Selects in falling order of 32-bit keys among candidates get(i, key), i < n, plus extra.ties more at extra.key, with
-  // `above` in front of them: the key T at which a rank ends and the number of candidates at T within it.  The
-  // rank takes candidates before which there are fewer than `limit` (kCount), or weight below `goal` (kBelow), or
-  // not above it (kUpTo).  Radix steps of up to 11 bits from the highest bit in which the candidates differ, each a
-  // histogram scanned from its largest bucket, until the candidates are equal.
-  enum { kCount, kBelow, kUpTo };
-  auto select = [&](int n, auto get, auto weight, u64 above, int rank, u64 limit, double goal, Cut extra, Cut none) {
+  // f(index, key) for the listed tokens (index in the list), and for all tokens of the row (eight loads in flight a thread).
+  auto list_key = [&](int i) { return (uint32_t)(list[i] >> 32); };
+  auto over_list = [&](auto&& f) {
+    for (int i = tid; i < (int)listed; i += kCutThreads) f(i, list_key(i));
+  };
+  auto over_row = [&](auto&& f) {
+    constexpr int kAhead = 8;
+    for (int i0 = tid; i0 < vocab; i0 += kAhead * kCutThreads) {
+      float v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j] = logit_at(x, min(i0 + j * kCutThreads, vocab - 1));
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kCutThreads < vocab) f(i0 + j * kCutThreads, order_key(v[j]));
+    }
+  };
+  // Selects in falling order of 32-bit keys among candidates, the (i, key) that `over` goes through and `has` accepts, plus
+  // extra.ties more at extra.key, with `above` in front of them: the key T at which a rank ends and the number of
+  // candidates at T within it.  The rank takes candidates before which there are fewer than `limit` (kCount), or
+  // weight below `goal` (kBelow).  Radix steps of up to 11 bits from the highest bit in which the candidates differ,
+  // each a histogram scanned from its largest bucket, until the candidates are equal.
+  enum { kCount, kBelow };
+  auto select = [&](auto over, auto has, auto weight, u64 above, int rank, u64 limit, double goal, Cut extra, Cut none) {
     int known = 32;  // candidates: key >> known == prefix
     uint32_t prefix = 0;
-    auto candidate = [&](int i, uint32_t& key) { return get(i, key) && (known == 32 || (key >> known) == prefix); };
-    auto within = [&](u64 v) { return rank == kCount ? v < limit : rank == kBelow ? (double)v < goal : !((double)v > goal); };
+    auto candidate = [&](int i, uint32_t key) { return has(i, key) && (known == 32 || (key >> known) == prefix); };
+    auto within = [&](u64 v) { return rank == kCount ? v < limit : (double)v < goal; };
     for (;;) {
       for (int i = tid; i < kBuckets; i += kCutThreads) hist[i] = 0, count[i] = 0;
       if (tid == 0) differ = 0u, sample_key = 0u, pick_step = 0xFFFFFFFFu;
       __syncthreads();
       const bool extra_now = extra.ties && (known == 32 || (extra.key >> known) == prefix);
-      uint32_t key, mine = 0, lo = 0xFFFFFFFFu;
-      for (int i = tid; i < n; i += kCutThreads)
+      uint32_t mine = 0, lo = 0xFFFFFFFFu;
+      over([&](int i, uint32_t key) {
         if (candidate(i, key)) mine = max(mine, key), lo = min(lo, key);
+      });
       if (extra_now && tid == 0) mine = max(mine, extra.key), lo = min(lo, extra.key);
       if (mine) atomicMax(&sample_key, mine);
       __syncthreads();
@@ -568,12 +588,12 @@ __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
       const uint32_t bits_off = differ;
       const int hb = bits_off ? 31 - __clz((int)bits_off) : -1, shift = max(0, hb - 10), bits = hb + 1 - shift;
       const uint32_t mask = bits ? (1u << bits) - 1u : 0u;
-      for (int i = tid; i < n; i += kCutThreads) {
-        if (!candidate(i, key)) continue;
+      over([&](int i, uint32_t key) {
+        if (!candidate(i, key)) return;
         const uint32_t bucket = (key >> shift) & mask;
         atomicAdd(&count[bucket], 1u);
         if (rank != kCount) atomicAdd(&hist[bucket], weight(i, key));
-      }
+      });
       __syncthreads();
       if (extra_now && tid == 0) {
         const uint32_t bucket = (extra.key >> shift) & mask;
@@ -623,34 +643,31 @@ __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
     }
   };
   auto key_weight = [&](int i, uint32_t key) { return need.listed ? list_weight[i] : r.fixed(logit_of_key(key)); };
-  auto list_key = [&](int i) { return (uint32_t)(list[i] >> 32); };
   // by counts: the first k of the tokens of the cut's step (the whole row without a list)
   auto top_k_cut = [&]() {
     const int step = need.k_step;
     if (need.listed)
-      return select((int)listed, [&](int i, uint32_t& key) { key = list_key(i); return r.step(logit_of_key(key)) == step; },
-                    key_weight, need.k_before, kCount, (u64)k, 0.0, Cut{0u, 0u}, cut);
-    return select(vocab, [&](int i, uint32_t& key) { key = order_key(logit_at(x, i)); return true; }, key_weight, 0, kCount,
-                  (u64)k, 0.0, Cut{0u, 0u}, cut);
+      return select(over_list, [&](int, uint32_t key) { return r.step(logit_of_key(key)) == step; }, key_weight, need.k_before,
+                    kCount, (u64)k, 0.0, Cut{0u, 0u}, cut);
+    return select(over_row, [](int, uint32_t) { return true; }, key_weight, 0, kCount, (u64)k, 0.0, Cut{0u, 0u}, cut);
   };
   // by weight: what is below `goal` of the tokens within `in` of a step (step < 0: of all listed, of the row without a list)
   auto top_p_cut = [&](int step, u64 before, double goal, Cut in) {
     if (need.listed)
-      return select((int)listed, [&](int i, uint32_t& key) {
-        key = list_key(i);
-        return key > in.key && (step < 0 || r.step(logit_of_key(key)) == step);
-      }, key_weight, before, kBelow, 0, goal, in, in);
-    return select(vocab, [&](int i, uint32_t& key) { key = order_key(logit_at(x, i)); return key > in.key; }, key_weight, 0,
-                  kBelow, 0, goal, in, in);
+      return select(over_list, [&](int, uint32_t key) { return key > in.key && (step < 0 || r.step(logit_of_key(key)) == step); },
+                    key_weight, before, kBelow, 0, goal, in, in);
+    return select(over_row, [&](int, uint32_t key) { return key > in.key; }, key_weight, 0, kBelow, 0, goal, in, in);
   };
   // weight of the listed tokens (of the row without a list) above the cut in a step (< 0: in all), and of its ties
   auto weight_of = [&](int step) {
     u64 part = 0, total;
-    const int n = need.listed ? (int)listed : vocab;
-    for (int i = tid; i < n; i += kCutThreads) {
-      const uint32_t key = need.listed ? list_key(i) : order_key(logit_at(x, i));
+    auto add = [&](int i, uint32_t key) {
       if (key > cut.key && (step < 0 || r.step(logit_of_key(key)) == step)) part += key_weight(i, key);
-    }
+    };
+    if (need.listed)
+      over_list(add);
+    else
+      over_row(add);
     if (tid == 0 && cut.ties) part += cut.ties * r.fixed(logit_of_key(cut.key));
     block_scan<kCutThreads>(part, red, total);
     return total;
@@ -698,11 +715,16 @@ __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
     for (int seg = tid >> 6; seg < s.segments; seg += kCutThreads / 64) {
       u64 sum = 0;
       uint32_t n = 0;
-      for (int i = seg * s.blocks_per_segment * kSegment + lane; i < min(vocab, (seg + 1) * s.blocks_per_segment * kSegment); i += 64) {
-        const float v = logit_at(x, i);
-        const uint32_t key = order_key(v);
-        if (key > cut.key) sum += kept_weight(r, v, least);
-        if (key == cut.key) ++n;
+      for (int blk = 0; blk < s.blocks_per_segment; ++blk) {
+        const int first = (seg * s.blocks_per_segment + blk) * kSegment + kLane * lane;
+        float v[kLane];
+        load_lane(x, first, vocab, v);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+          const uint32_t key = order_key(v[j]);
+          if (key > cut.key) sum += kept_weight(r, v[j], least);
+          if (first + j < vocab && key == cut.key) ++n;
+        }
       }
       sum = wave_sum(sum);
       n = wave_sum(n);
