@@ -9,8 +9,8 @@
 // which they cut, and of each segment of the row the weight of the tokens in steps that are kept whatever the cut; the
 // exact (T, n) from the list, and the draw: the listed tokens that are kept join their segments, the goal is found in
 // the segments' running sum and then among the tokens of one segment.  Rows are split over many blocks except in
-// the last launch.  A row with a small k lists everything down to the step of its cut: its weights are those of
-// the list only.
+// the last launch.  A row with a small k and a top-p lists everything down to the step of its cut: its weights are
+// those of the list only.
 #include <hip/hip_runtime.h>
 
 #include "kernels.hpp"
@@ -23,7 +23,10 @@ namespace {
 constexpr int kBuckets = 2048;
 constexpr int kList = 4096;     // most tokens that are listed (more: radix steps over the whole row; 151936 normal
                                 // logits have up to 270 in a step)
-constexpr int kSmall = 2048;    // largest k whose row is decided by its list
+// Largest k whose row is decided by its list where there is a top-p too, without weights in the histogram.  151936 tokens
+// with a top-p, this way and by the histogram: k = 200 35 us and 36, 64 rows 64 and 80; k = 1000 44 and 41, 73 and 87;
+// k = 2000 51 and 42, 82 and 91.  (Without a top-p the list takes longer: k = 200 25.0 and 24.7, k = 2000 35 and 30.)
+constexpr int kSmall = 1024;
 constexpr int kSegment = 512;   // tokens of a segment (times 2, 3, .. for more than kMaxSegments * 512 tokens)
 constexpr int kMaxSegments = 1024;
 constexpr int kMaxChunks = 256;
@@ -275,7 +278,7 @@ __device__ __forceinline__ bool wants_top_k(const Sampler& s, int row, int& k) {
   k = s.a.top_k ? s.a.top_k[row] : 0;
   return k > 0 && k < s.a.vocab;
 }
-__device__ __forceinline__ bool small_k(bool top_k, int k) { return top_k && k <= kSmall; }
+__device__ __forceinline__ bool small_k(bool top_k, int k, bool top_p) { return top_k && k <= kSmall && top_p; }
 __device__ __forceinline__ bool wants_top_p(const Sampler& s, int row, float& p) {
   p = s.a.top_p ? s.a.top_p[row] : 1.0f;
   return p < 1.0f;
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(kHistThreads) sample_hist_kernel(Sampler s) {
   float p;
   const bool top_p = wants_top_p(s, row, p), top_k = wants_top_k(s, row, k);
   if (!top_k && !top_p) return;
-  const bool weigh = top_p && !small_k(top_k, k);
+  const bool weigh = top_p && !small_k(top_k, k, top_p);
   const Row r(s, row, red);
   if (r.greedy) return;
   for (int i = tid; i < kBuckets; i += kHistThreads) weights[i] = 0, counts[i] = 0;
@@ -393,7 +396,7 @@ __device__ Needed needed_steps(const Held<N>& h, bool top_k, int k, bool top_p, 
   if (top_k) {
     const auto f = h.find(false, (u64)k, 0.0, kBuckets, 0, pick, pick_step);
     if (f.step < kBuckets - 1) n.k_step = f.step, n.k_before = f.before, at = f.at, tokens = f.tokens;
-    if (small_k(top_k, k)) {  // everything with weight down to the cut
+    if (small_k(top_k, k, top_p)) {  // everything with weight down to the cut
       n.low = 0, n.high = min(f.step, kBuckets - 2);
       n.listed = f.before + tokens <= (u64)kList;
       return n;
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(kHistThreads) sample_list_kernel(Sampler s) {
   if (top_k || top_p) {
     held.scan(red);
     need = needed_steps(held, top_k, k, top_p, p, pick, &pick_step);
-    if (top_p || small_k(top_k, k))
+    if (top_p)
       sure = need.low;
     else if (need.k_step >= 0)
       sure = need.k_step;
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kCutThreads) sample_cut_kernel(Sampler s) {
   RowSpace& w = s.space[row];
   const uint32_t listed = w.listed;
   Needed need{w.k_step, w.p_low, w.p_high, w.k_before, listed != kUnlisted};
-  const bool small = small_k(top_k, k);
+  const bool small = small_k(top_k, k, top_p);
   const float uf = s.a.uniforms[row];
   const double least = least_weight(s, row);
   Held<kCutThreads> held(w);
