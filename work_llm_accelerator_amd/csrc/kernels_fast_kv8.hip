@@ -618,8 +618,10 @@ void launch_fill_i32(int* p, int n, int value, hipStream_t st) {
 // - Up to four tiles of 16 columns go to the kernel that reads the cache into registers, two of them a workgroup, more to
 //   the kernel of large tiles: 64 sequences of 4000 tokens with 5 fp32 rows (four tiles) 47 us, as a large tile 68; with 6
 //   rows (five) 81 and 70.
-// - Few rows: keys split to one workgroup a CU (512, 768 or 1024 of them: slower, by their joins), in whole turns of the
-//   four waves.  A sequence of up to 12 blocks is not split: three blocks a wave cost less than the second launch.
+// - Few rows: keys split to one workgroup a CU or a few more (twice as many: 64 sequences of 4096 tokens the same, 16 of 8000
+//   10 % more, 100 of 50 to 3000 tokens 10 % less), in equal parts (100 sequences of 3000 tokens 31 us; in one part of 40
+//   blocks and one of 7, 41) of whole turns of the four waves.  A sequence of up to 12 blocks is not split: three blocks
+//   a wave cost less than the second launch.
 // - Large tiles: keys split so that the workgroups come to one a CU at most, two blocks or more each (512 rows after 32000
 //   tokens of one sequence: 203 us (129); one a CU or a little more, which leaves some CUs two: 242 (158)).
 // - Several key groups a workgroup where each workgroup has a CU to itself and 12 blocks or more (28 / 4 heads of 64, 204
@@ -646,7 +648,8 @@ Kv8AttnPlan plan_kv8_attention(const qwen_kv8_cache& c, int type, int q_heads, i
   } else {
     per = (blocks * others + kCus - 1) / kCus;
     if (per < 4) per = blocks <= 12 ? blocks : 4;
-    per = (per + 3) / 4 * 4;
+    const long long splits = (blocks + per - 1) / per;
+    per = ((blocks + splits - 1) / splits + 3) / 4 * 4;
   }
   const long long least = (blocks + kKv8MaxSplits - 1) / kKv8MaxSplits;
   if (per < least) per = least;

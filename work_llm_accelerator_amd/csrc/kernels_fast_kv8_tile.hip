@@ -350,15 +350,15 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(K
       if constexpr (KG > 2) tick();
       probabilities(std::integral_constant<int, 1>{});
       l += __builtin_amdgcn_ldexpf(sum, shift);
+      write_v();
+      write_k();
+      sk = a.c.k_scale[place(it + 1)];
+      svf = a.c.v_scale[place(it + 1)];
       if (__any(drop))
 #pragma unroll
         for (int b2 = 0; b2 < kLimbs; ++b2)
 #pragma unroll
           for (int u = 0; u < 4; ++u) p[b2][u] = drop ? half8{} : p[b2][u];
-      write_v();
-      write_k();
-      sk = a.c.k_scale[place(it + 1)];
-      svf = a.c.v_scale[place(it + 1)];
       tick();
       weigh();
     }
