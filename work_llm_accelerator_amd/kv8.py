@@ -49,9 +49,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_HERE = nullcontext()
+
+
 def _on(device):
     """A context in which `device` is the current one."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)
 
 
 @dataclass
@@ -114,24 +118,24 @@ class Kv8Cache:
                                   self.k_scale.data_ptr() + 4 * n, self.v_scale.data_ptr() + 4 * n, sequences, blocks,
                                   heads, width // BLOCK)
 
-    def _rows(self, t, shape: tuple, what: str) -> abi.Kv8RowsStruct:
-        """`t` of `shape` as qwen_kv8_rows."""
+    def _rows(self, t, shape: tuple, device, what: str) -> abi.Kv8RowsStruct:
+        """`t` of `shape` on `device` as qwen_kv8_rows."""
         strides = t.stride()
         if t.shape != shape:
             raise ValueError(f"{what} must be {shape}, not {tuple(t.shape)}")
-        if shape[0] > MAX_COUNT or shape[1] > MAX_COUNT or shape[2] > MAX_COUNT:  # (ctypes would cut them to 32 bits)
+        if max(shape) > MAX_COUNT:  # (ctypes would cut it to 32 bits)
             raise ValueError(f"{what} has a dimension above {MAX_COUNT}")
-        if t.device != self.k.device:
-            raise ValueError(f"{what} must be on {self.k.device}, not {t.device}")
+        if t.device != device:
+            raise ValueError(f"{what} must be on {device}, not {t.device}")
         if strides[3] != 1:
             raise ValueError(f"{what}: the values of a row must be contiguous")
         return abi.Kv8RowsStruct(t.data_ptr(), strides[0], strides[1], strides[2])
 
-    def _positions(self, positions, batch: int) -> int:
+    def _positions(self, positions, batch: int, device) -> int:
         if positions.dtype != torch.int32 or positions.shape != (batch,) or not positions.is_contiguous():
             raise ValueError(f"positions must be {batch} contiguous int32 values")
-        if positions.device != self.k.device:
-            raise ValueError(f"positions must be on {self.k.device}, not {positions.device}")
+        if positions.device != device:
+            raise ValueError(f"positions must be on {device}, not {positions.device}")
         return positions.data_ptr()
 
     def store(self, layer: int, k, v, positions) -> None:
@@ -143,12 +147,13 @@ class Kv8Cache:
         if k.dtype != v.dtype:
             raise ValueError("k and v must have one type")
         batch, rows = k.shape[:2]
-        shape = (batch, rows, self.kv_heads, self.head_dim)
-        ks, vs = self._rows(k, shape, "k"), self._rows(v, shape, "v")
-        pos, c, lib = self._positions(positions, batch), self.layer_struct(layer), abi.load()
-        with _on(self.k.device):
+        c, lib, device = self.layer_struct(layer), abi.load(), self.k.device
+        shape = (batch, rows, c.kv_heads, c.head_dim)
+        ks, vs = self._rows(k, shape, device, "k"), self._rows(v, shape, device, "v")
+        pos = self._positions(positions, batch, device)
+        with _on(device):
             st = lib.qwen_hip_kv8_store(ctypes.byref(c), _type_of(k), ctypes.byref(ks), ctypes.byref(vs), batch, rows,
-                                        pos, _raw_stream(self.k.device.index))
+                                        pos, _raw_stream(device.index))
         _check(lib, st, "qwen_hip_kv8_store")
 
     def load(self, layer: int, positions, rows: int | None = None, k=None, v=None, dtype=None):
@@ -169,12 +174,13 @@ class Kv8Cache:
         if k.dtype != v.dtype:
             raise ValueError("k and v must have one type")
         batch, rows = k.shape[:2]
-        shape = (batch, rows, self.kv_heads, self.head_dim)
-        ks, vs = self._rows(k, shape, "k"), self._rows(v, shape, "v")
-        pos, c, lib = self._positions(positions, batch), self.layer_struct(layer), abi.load()
-        with _on(self.k.device):
+        c, lib, device = self.layer_struct(layer), abi.load(), self.k.device
+        shape = (batch, rows, c.kv_heads, c.head_dim)
+        ks, vs = self._rows(k, shape, device, "k"), self._rows(v, shape, device, "v")
+        pos = self._positions(positions, batch, device)
+        with _on(device):
             st = lib.qwen_hip_kv8_load(ctypes.byref(c), _type_of(k), ctypes.byref(ks), ctypes.byref(vs), batch, rows,
-                                       flags, pos, _raw_stream(self.k.device.index))
+                                       flags, pos, _raw_stream(device.index))
         _check(lib, st, "qwen_hip_kv8_load")
         return k, v
 
@@ -190,22 +196,22 @@ class Kv8Cache:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if out.dtype != q.dtype:
             raise ValueError("q and out must have one type")
-        max_keys = int(max_keys)
-        if not 0 < max_keys <= self.positions:
-            raise ValueError(f"max_keys must be 1 .. {self.positions}, not {max_keys}")
-        shape = (batch, rows, heads, self.head_dim)
-        qs, os = self._rows(q, shape, "q"), self._rows(out, shape, "out")
-        pos, c, lib, kind = self._positions(positions, batch), self.layer_struct(layer), abi.load(), _type_of(q)
+        max_keys, c, lib, kind, device = int(max_keys), self.layer_struct(layer), abi.load(), _type_of(q), self.k.device
+        if not 0 < max_keys <= BLOCK * c.blocks:
+            raise ValueError(f"max_keys must be 1 .. {BLOCK * c.blocks}, not {max_keys}")
+        shape = (batch, rows, heads, c.head_dim)
+        qs, os = self._rows(q, shape, device, "q"), self._rows(out, shape, device, "out")
+        pos = self._positions(positions, batch, device)
         need = ctypes.c_uint64(0)
-        with _on(self.k.device):
+        with _on(device):
             _check(lib, lib.qwen_hip_kv8_attention_workspace(ctypes.byref(c), kind, heads, batch, rows, max_keys,
                                                              ctypes.byref(need)), "qwen_hip_kv8_attention_workspace")
             # the stream's own allocation: reused by later work of this stream only, private to a graph being captured
-            ws = torch.empty(need.value, dtype=torch.uint8, device=self.k.device) if need.value else None
+            ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
             st = lib.qwen_hip_kv8_attention(ctypes.byref(c), kind, ctypes.byref(qs), ctypes.byref(os), heads, batch, rows,
                                             pos, max_keys, 1.0 / math.sqrt(self.head_dim) if scale is None else scale,
                                             ws.data_ptr() if ws is not None else None, need.value,
-                                            _raw_stream(self.k.device.index))
+                                            _raw_stream(device.index))
         _check(lib, st, "qwen_hip_kv8_attention")
         return out
 
